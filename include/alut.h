@@ -36,6 +36,9 @@
  *   alut_route            table_moe/ops/qwen_topk_softmax.py:122-153 + cached_layers.py:69-84
  *   alut_keep_mask        table_moe/skip/pruning.py:18-48 build_prefill_keep_mask
  *   alut_normalize_rows   table_moe/cache_engine/manager.py:24-31, :205-207
+ *   alut_route_experts / alut_quantize_fp8 / alut_linear_fp8 / alut_experts_fp8
+ *                         new: expert routing with sigmoid scores, a balance bias and groups, and
+ *                         the computed experts (cached_layers.py:431-437 leaves them to a loop)
  *   alut_search_packed /
  *   alut_merge_packed     centroid-range sharding of one large table (new: the reference
  *                         is single-GPU; the merge rule is the tie rule of search.py:89)
@@ -359,6 +362,94 @@ int alut_route(int32_t q, int32_t num_experts, int32_t top_k, const void* logits
 int alut_keep_mask(int32_t q, int32_t num_experts, int32_t top_k, const int64_t* sel, const float* weights,
                    int64_t in_stride, const float* attn, double keep_rate, uint8_t* compute, uint8_t* reuse,
                    int64_t out_stride, void* workspace, size_t workspace_bytes, alut_stream_t stream);
+
+/* ---- routed experts beyond the lookup (new: the reference routes by a plain softmax and leaves
+ * the computed experts to its caller's loop, cached_layers.py:280-337, :431-437) -------------- */
+
+typedef enum alut_scoring {
+  ALUT_SCORE_SOFTMAX = 0,
+  ALUT_SCORE_SIGMOID = 1,
+} alut_scoring_t;
+
+typedef enum alut_group_rule {
+  ALUT_GROUP_MAX = 0,  /* a group counts by its largest key */
+  ALUT_GROUP_TOP2 = 1, /* ... by the sum of its two largest keys */
+} alut_group_rule_t;
+
+/* How alut_route_experts chooses. Experts form n_group groups of num_experts / n_group
+ * consecutive ones; n_group <= 32 and topk_group * (num_experts / n_group) >= top_k. */
+typedef struct alut_router {
+  int32_t num_experts;
+  int32_t top_k;
+  int32_t scoring;      /* alut_scoring_t */
+  int32_t n_group;      /* 1: no groups */
+  int32_t topk_group;
+  int32_t group_rule;   /* alut_group_rule_t */
+  int32_t normalize_topk;
+  float scale;          /* multiplies the weights, after the normalisation */
+  const float* bias;    /* [num_experts] or NULL: added to the scores for the choice only; finite */
+} alut_router_t;
+
+/* Routing of q tokens and the keep mask of alut_route (same keep modes, outputs, strides and
+ * workspace). Scores p = softmax(logits) or 1 / (1 + exp(-logits)); the choice is by key =
+ * p + bias, or by the logit itself when there is no bias and groups go by their largest key
+ * (the same order); NaN keys and -inf logits rank last, the lowest expert id first among equal
+ * keys; the topk_group best groups, then the top_k largest keys in them, in descending order.
+ * weights = p of the chosen, over max(their sum, 1e-20) with normalize_topk, times scale; a
+ * softmax row of only -inf has scores 0. */
+int alut_route_experts(const alut_router_t* router, int32_t q, const void* logits, int32_t logits_dtype,
+                       int64_t logits_stride, int32_t keep_mode, int32_t keep_k, double keep_rate, const float* attn,
+                       float* weights, int64_t* sel, uint8_t* compute, uint8_t* reuse, int64_t out_stride,
+                       void* workspace, size_t workspace_bytes, alut_stream_t stream);
+
+/* The 8-bit form used below: e4m3 numbers with one fp32 scale per block. Per block
+ *   a = max(max |src|, 2^-100), scale = a / 448, out = e4m3(src * (448 / a)), all in fp32;
+ * a block with a NaN or an infinity stands for NaN. block_rows 1: a block is 128 columns of one
+ * row (activations); 128: 128 rows x 128 columns (weights). Blocks at the edges are short.
+ * src is [batch][rows][cols] (dtype, element strides, unit innermost), out bytes with byte
+ * strides, scale contiguous fp32 [batch][ceil(rows / block_rows)][ceil(cols / 128)]. */
+int alut_quantize_fp8(int64_t batch, int64_t rows, int32_t cols, int32_t block_rows, const void* src, int32_t dtype,
+                      int64_t src_stride_b, int64_t src_stride, void* out, int64_t out_stride_b, int64_t out_stride,
+                      float* scale, alut_stream_t stream);
+
+/* out[m, n] = x[m, k] . w[n, k]^T with w e4m3 (16-byte aligned, row stride w_stride a multiple of
+ * 16 bytes and >= ceil(k / 16) * 16; what lies past column k is never used) and its scales
+ * contiguous fp32 [ceil(n / 128)][ceil(k / 128)]. x (f32/bf16/f16) is taken in its 8-bit form,
+ * one scale per row and 128 columns, made inside the call. Products and sums are fp32; out has
+ * out_dtype, any row stride >= n. error_bits (device, may be NULL) collects ALUT_ERR_*. */
+size_t alut_linear_fp8_workspace_size(int32_t m, int32_t n, int32_t k);
+int alut_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, int32_t x_dtype, int64_t x_stride, const void* w,
+                    int64_t w_stride, const float* w_scale, void* out, int32_t out_dtype, int64_t out_stride,
+                    uint32_t* error_bits, void* workspace, size_t workspace_bytes, alut_stream_t stream);
+
+/* The experts of a layer: down(silu(gate . x) * (up . x)). Weights e4m3 with the rules of
+ * alut_linear_fp8; all strides are multiples of 16 bytes. */
+typedef struct alut_fp8_experts {
+  int32_t num_experts; /* E <= 2048 */
+  int32_t h;           /* H, hidden size */
+  int32_t i;           /* I, the experts' inner size */
+  int32_t reserved0;
+  const void* gate_up;         /* [E][2][I][H]: gate rows, then up rows */
+  int64_t gate_up_stride[3];   /* bytes: expert, half, row */
+  const float* gate_up_scale;  /* contiguous [E][2][ceil(I / 128)][ceil(H / 128)] */
+  const void* down;            /* [E][H][I] */
+  int64_t down_stride[2];      /* bytes: expert, row */
+  const float* down_scale;     /* contiguous [E][ceil(H / 128)][ceil(I / 128)] */
+} alut_fp8_experts_t;
+
+/* The computed slots' experts: for every slot with compute[t, s] (NULL: all),
+ *   out[t, s, :] = down_e(silu(gate_e x[t]) * (up_e x[t])), e = sel[t, s],
+ * the rows that alut_lookup_combine_experts takes as `computed`. x and the inner activations
+ * are taken in their 8-bit form (one scale per row and 128 columns); everything else is fp32.
+ * Rows of other slots are set to 0 with zero_skipped and left alone without. A computed slot
+ * whose expert id is outside [0, E) counts as not computed and sets ALUT_ERR_BAD_EXPERT in
+ * error_bits (device, may be NULL). The workspace needs no initial contents. */
+size_t alut_experts_fp8_workspace_size(const alut_fp8_experts_t* experts, int32_t q, int32_t s);
+int alut_experts_fp8(const alut_fp8_experts_t* experts, int32_t q, int32_t s, const void* x, int32_t x_dtype,
+                     int64_t x_stride, const int64_t* sel, int64_t sel_stride, const uint8_t* compute,
+                     int64_t compute_stride, int32_t zero_skipped, void* out, int32_t out_dtype, int64_t out_stride_t,
+                     int64_t out_stride_s, uint32_t* error_bits, void* workspace, size_t workspace_bytes,
+                     alut_stream_t stream);
 
 /* Load-time key normalisation (table_moe/cache_engine/manager.py:24-31, :205-207): for each
  * of `rows` rows of l elements (dtype, row strides in elements; dst may equal src)

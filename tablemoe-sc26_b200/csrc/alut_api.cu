@@ -11,6 +11,7 @@
 
 #include "alut_combine.cuh"
 #include "alut_common.cuh"
+#include "alut_host.cuh"
 #include "alut_project.cuh"
 #include "alut_search.cuh"
 #include "alut_tc.cuh"
@@ -18,21 +19,13 @@
 #include "alut_peer.cuh"
 #include "alut_online.cuh"
 #include "alut_route.cuh"
+#include "alut_route_experts.cuh"
 
 namespace alut {
 
 static void* noalloc_scratch_ptr(int* rc);
-static thread_local char g_err[512] = "no error";
 static thread_local cudaEvent_t g_prof_start = nullptr;
 static thread_local cudaEvent_t g_prof_stop = nullptr;
-
-static int fail(int code, const char* fmt, ...) {
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(g_err, sizeof(g_err), fmt, ap);
-  va_end(ap);
-  return code;
-}
 
 // Records a profiling event (alut_set_profile_events) around the scan: as an external event
 // node while the stream is being captured into a graph, as a plain record otherwise.
@@ -47,51 +40,10 @@ static int record_profile(cudaEvent_t ev, cudaStream_t st) {
   return ALUT_OK;
 }
 
-static int check_launch(const char* what) {
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return fail(ALUT_ECUDA, "%s: %s", what, cudaGetErrorString(e));
-  return ALUT_OK;
-}
-
 float host_round_as(float v, int dtype) {
   if (dtype == ALUT_BF16) return __bfloat162float(__float2bfloat16_rn(v));
   if (dtype == ALUT_F16) return __half2float(__float2half_rn(v));
   return v;
-}
-
-static int dtype_size(int d) { return d == ALUT_F32 ? 4 : 2; }
-static bool dtype_ok(int d) { return d == ALUT_F32 || d == ALUT_BF16 || d == ALUT_F16; }
-static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-static int num_sms() {
-  static int cache[64] = {0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return 148;
-  if (dev < 64 && cache[dev]) return cache[dev];
-  int n = 148;
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) n = 148;
-  if (dev < 64) cache[dev] = n;
-  return n;
-}
-
-// Raise a kernel's dynamic shared memory limit once per (kernel, device).
-static int allow_smem(const void* kernel, size_t bytes) {
-  if (bytes <= 48 * 1024) return ALUT_OK;
-  struct Entry { const void* k; int dev; int bytes; };
-  static Entry table[256];
-  static int used = 0;
-  static std::mutex mu;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  std::lock_guard<std::mutex> lock(mu);
-  for (int i = 0; i < used; ++i)
-    if (table[i].k == kernel && table[i].dev == dev && table[i].bytes >= static_cast<int>(bytes))
-      return ALUT_OK;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(bytes));
-  if (e != cudaSuccess) return fail(ALUT_ECUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-  if (used < 256) table[used++] = Entry{kernel, dev, static_cast<int>(bytes)};
-  return ALUT_OK;
 }
 
 static size_t basis_plain_bytes(int l, int h) { return static_cast<size_t>(2) * 3 * l * h * sizeof(__nv_bfloat16); }
@@ -152,24 +104,6 @@ static int check_params(const alut_tables_t* t, const alut_search_params_t* p, c
 }
 
 // ---- launches ------------------------------------------------------------------------
-
-// Launch as a programmatic dependent of the previous kernel in the stream (it may start
-// early and waits in griddepcontrol.wait for the predecessor's results).
-template <typename... KArgs, typename... Args>
-static cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
-                              cudaStream_t st, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
 
 // Projection: grid = qtiles x nsplit CTAs; the nsplit CTAs of a token tile form one
 // thread-block cluster (they add their partial tiles through distributed shared memory).
@@ -867,6 +801,83 @@ int alut_route(int32_t q, int32_t num_experts, int32_t top_k, const void* logits
   rc = check_launch("k_route_topk");
   if (rc || keep_mode != ALUT_KEEP_IMPORTANCE) return rc;
   const size_t ks = (sizeof(long long) + sizeof(int) + 1) * static_cast<size_t>(num_experts);
+  rc = allow_smem(reinterpret_cast<const void*>(k_route_keep), ks);
+  if (rc) return rc;
+  k_route_keep<<<1, kRouteKeepThreads, ks, st>>>(a);
+  return check_launch("k_route_keep");
+}
+
+int alut_route_experts(const alut_router_t* router, int32_t q, const void* logits, int32_t logits_dtype,
+                       int64_t logits_stride, int32_t keep_mode, int32_t keep_k, double keep_rate, const float* attn,
+                       float* weights, int64_t* sel, uint8_t* compute, uint8_t* reuse, int64_t out_stride,
+                       void* workspace, size_t workspace_bytes, alut_stream_t stream) {
+  if (!router) return fail(ALUT_EINVAL, "route_experts: router is NULL");
+  const int E = router->num_experts, k = router->top_k, G = router->n_group, tg = router->topk_group;
+  if (q < 0 || E <= 0 || k <= 0 || G <= 0 || tg <= 0)
+    return fail(ALUT_EINVAL, "route_experts: q=%d experts=%d top_k=%d n_group=%d topk_group=%d", q, E, k, G, tg);
+  if (E > kRouteMaxExperts || k > kMaxSlots || k > E)
+    return fail(ALUT_ERANGE, "route_experts: top_k=%d must be <= min(64, experts) and experts=%d <= %d", k, E,
+                kRouteMaxExperts);
+  if (G > kRouteMaxGroups || E % G != 0 || tg > G)
+    return fail(ALUT_ERANGE, "route_experts: n_group=%d must be <= %d and divide experts=%d, topk_group=%d <= n_group", G,
+                kRouteMaxGroups, E, tg);
+  if (static_cast<int64_t>(tg) * (E / G) < k)
+    return fail(ALUT_ERANGE, "route_experts: %d groups of %d experts hold fewer than top_k=%d", tg, E / G, k);
+  if ((router->scoring != ALUT_SCORE_SOFTMAX && router->scoring != ALUT_SCORE_SIGMOID) ||
+      (router->group_rule != ALUT_GROUP_MAX && router->group_rule != ALUT_GROUP_TOP2))
+    return fail(ALUT_EINVAL, "route_experts: scoring or group rule");
+  if (!dtype_ok(logits_dtype)) return fail(ALUT_EDTYPE, "route_experts: logits dtype");
+  if (keep_mode != ALUT_KEEP_FIXED && keep_mode != ALUT_KEEP_IMPORTANCE)
+    return fail(ALUT_EINVAL, "route_experts: keep mode");
+  if (q == 0) return ALUT_OK;
+  if (!logits || !weights || !sel || !compute || !reuse) return fail(ALUT_EINVAL, "route_experts: NULL argument");
+  if (logits_stride < E || out_stride < k) return fail(ALUT_ESHAPE, "route_experts: strides");
+  const size_t need = alut_route_workspace_size(E);
+  if (keep_mode == ALUT_KEEP_IMPORTANCE && (!workspace || workspace_bytes < need))
+    return fail(ALUT_EWORKSPACE, "route_experts: workspace has %zu bytes, needs %zu", workspace_bytes, need);
+  if (keep_mode == ALUT_KEEP_IMPORTANCE && !(keep_rate >= 0.0))
+    return fail(ALUT_EINVAL, "route_experts: keep_rate must be >= 0");
+  RouteExpertsArgs x{};
+  RouteArgs& a = x.r;
+  a.q = q;
+  a.e = E;
+  a.k = k;
+  a.logits = logits;
+  a.logits_dtype = logits_dtype;
+  a.logits_stride = logits_stride;
+  a.normalize = router->normalize_topk;
+  a.mode = keep_mode;
+  a.keep_k = keep_k < 0 ? k : std::min(keep_k, k);
+  a.keep_rate = keep_rate;
+  a.attn = attn;
+  a.w = weights;
+  a.sel = sel;
+  a.compute = compute;
+  a.reuse = reuse;
+  a.out_stride = out_stride;
+  if (workspace) {
+    a.sums = static_cast<unsigned long long*>(workspace);
+    a.counts = reinterpret_cast<int*>(static_cast<char*>(workspace) + align256(sizeof(unsigned long long) * E));
+  }
+  x.bias = router->bias;
+  x.sigmoid = router->scoring == ALUT_SCORE_SIGMOID;
+  x.n_group = G;
+  x.topk_group = tg;
+  x.top2 = router->group_rule == ALUT_GROUP_TOP2;
+  x.scale = router->scale;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  void (*kern)(RouteExpertsArgs) = E <= 64    ? k_route_experts<2>
+                                   : E <= 128 ? k_route_experts<4>
+                                   : E <= 256 ? k_route_experts<8>
+                                   : E <= 512 ? k_route_experts<16>
+                                              : k_route_experts<0>;
+  const size_t sm = sizeof(float) * 2 * kRouteWarps * E;
+  int rc = allow_smem(reinterpret_cast<const void*>(kern), sm);
+  if (rc) return rc;
+  kern<<<ceil_div(q, kRouteWarps), kRouteWarps * 32, sm, st>>>(x);
+  rc = check_launch("k_route_experts");
+  if (rc || keep_mode != ALUT_KEEP_IMPORTANCE) return rc;
+  const size_t ks = (sizeof(long long) + sizeof(int) + 1) * static_cast<size_t>(E);
   rc = allow_smem(reinterpret_cast<const void*>(k_route_keep), ks);
   if (rc) return rc;
   k_route_keep<<<1, kRouteKeepThreads, ks, st>>>(a);

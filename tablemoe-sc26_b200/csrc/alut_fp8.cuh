@@ -1,0 +1,491 @@
+// 8-bit floating point (e4m3) products with a scale for each block of 128: the number form,
+// its quantisers, the plan that groups routed slots by expert, and the weight-streaming
+// product for few rows.
+//
+// The form. A row x is cut into blocks of 128 columns (the last one short). Per block, in
+// fp32: a = max(max|x|, 2^-100), scale s = a / 448, factor f = 448 / a, q = e4m3(x f) (round
+// to nearest even; |x f| <= 448 up to one rounding, which e4m3 rounds back to 448). A NaN or
+// an infinity in a block makes the whole block's products NaN: a is a maximum of bit patterns,
+// which NaN wins, and inf * 0 is NaN. A weight [N, K] has one scale per 128 x 128 block.
+//
+// A product is y[m, n] = sum_B sx[m, B] sw[n / 128, B] (sum_{k in B} qx[m, k] qw[n, k]): the
+// inner sum runs on tensor cores (products of two e4m3 numbers are exact in fp32), the outer
+// one in fp32 registers, once per block.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "alut_common.cuh"
+
+namespace alut {
+
+constexpr int kFp8Block = 128;
+constexpr float kE4m3Max = 448.0f;
+constexpr float kFp8AmaxFloor = 7.888609052210118e-31f;  // 2^-100: 448 / a stays finite
+
+__host__ __device__ inline int fp8_blocks(int n) { return (n + kFp8Block - 1) / kFp8Block; }
+
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// The block's largest magnitude from the largest bit pattern (NaN patterns are the largest).
+__device__ __forceinline__ float fp8_amax(uint32_t bits) {
+  const float a = __uint_as_float(bits);
+  return a < kFp8AmaxFloor ? kFp8AmaxFloor : a;
+}
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  return e4m3x2(a, b) | (e4m3x2(c, d) << 16);
+}
+
+// Runtime-typed element access (quantisers' inputs, ragged edges, outputs).
+__device__ __forceinline__ float load_any(const void* p, int64_t i, int dtype) {
+  if (dtype == ALUT_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  if (dtype == ALUT_F16) return __half2float(static_cast<const __half*>(p)[i]);
+  return static_cast<const float*>(p)[i];
+}
+__device__ __forceinline__ void store_any(void* p, int64_t i, float v, int dtype) {
+  if (dtype == ALUT_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else if (dtype == ALUT_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
+  else static_cast<float*>(p)[i] = v;
+}
+
+// ---- quantisers ------------------------------------------------------------------------------
+
+struct QuantArgs {
+  int64_t batch, rows;
+  int cols, dtype;
+  const void* src;
+  int64_t src_stride_b, src_stride;  // elements
+  uint8_t* out;
+  int64_t out_stride_b, out_stride;  // bytes
+  float* scale;                       // contiguous [batch][row blocks][column blocks]
+};
+
+// One scale per row and 128 columns: a warp per block, four consecutive columns per lane.
+__global__ void __launch_bounds__(256) k_fp8_quantize_rows(QuantArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int kb = fp8_blocks(a.cols);
+  const int64_t n = a.batch * a.rows * kb;
+  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; i < n;
+       i += (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5) {
+    const int b = static_cast<int>(i % kb);
+    const int64_t row = i / kb;
+    const int64_t so = (row / a.rows) * a.src_stride_b + (row % a.rows) * a.src_stride;
+    const int64_t oo = (row / a.rows) * a.out_stride_b + (row % a.rows) * a.out_stride;
+    const int c0 = b * kFp8Block + lane * 4;
+    float v[4];
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = c0 + j < a.cols ? load_any(a.src, so + c0 + j, a.dtype) : 0.f;
+      m = max(m, abs_bits(v[j]));
+    }
+    const float am = fp8_amax(__reduce_max_sync(0xffffffffu, m));
+    const float f = kE4m3Max / am;
+    const uint32_t q = e4m3x4(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c0 + j < a.cols) a.out[oo + c0 + j] = static_cast<uint8_t>(q >> (8 * j));
+    if (lane == 0) a.scale[i] = am / kE4m3Max;
+  }
+}
+
+// One scale per 128 x 128 block (weights): a CTA per block.
+__global__ void __launch_bounds__(256) k_fp8_quantize_blocks(QuantArgs a) {
+  __shared__ uint32_t s_max;
+  const int kb = fp8_blocks(a.cols);
+  const int64_t rb = (a.rows + kFp8Block - 1) / kFp8Block;
+  const int64_t n = a.batch * rb * kb;
+  for (int64_t i = blockIdx.x; i < n; i += gridDim.x) {
+    const int64_t bi = i / (rb * kb), ri = (i / kb) % rb;
+    const int ci = static_cast<int>(i % kb);
+    const int64_t r0 = ri * kFp8Block;
+    const int nr = static_cast<int>(min(static_cast<int64_t>(kFp8Block), a.rows - r0));
+    const int nc = min(kFp8Block, a.cols - ci * kFp8Block);
+    const int64_t so = bi * a.src_stride_b + r0 * a.src_stride + ci * kFp8Block;
+    const int64_t oo = bi * a.out_stride_b + r0 * a.out_stride + ci * kFp8Block;
+    if (threadIdx.x == 0) s_max = 0;
+    __syncthreads();
+    uint32_t m = 0;
+    for (int e = threadIdx.x; e < kFp8Block * kFp8Block; e += blockDim.x) {
+      const int r = e >> 7, c = e & 127;
+      if (r < nr && c < nc) m = max(m, abs_bits(load_any(a.src, so + r * a.src_stride + c, a.dtype)));
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if ((threadIdx.x & 31) == 0) atomicMax(&s_max, m);
+    __syncthreads();
+    const float am = fp8_amax(s_max);
+    const float f = kE4m3Max / am;
+    for (int e = threadIdx.x; e < kFp8Block * kFp8Block; e += blockDim.x) {
+      const int r = e >> 7, c = e & 127;
+      if (r < nr && c < nc)
+        a.out[oo + r * a.out_stride + c] =
+            static_cast<uint8_t>(e4m3x2(load_any(a.src, so + r * a.src_stride + c, a.dtype) * f, 0.f));
+    }
+    if (threadIdx.x == 0) a.scale[i] = am / kE4m3Max;
+    __syncthreads();
+  }
+}
+
+// ---- plan: computed slots grouped by expert ---------------------------------------------------
+
+struct Fp8Route {
+  int q, s, e;
+  const int64_t* sel;
+  int64_t sel_stride;
+  const uint8_t* compute;  // NULL: every slot
+  int64_t compute_stride;
+  uint32_t* err;
+};
+
+// The expert of slot i, or -1 if the slot is not computed (or names no expert).
+__device__ __forceinline__ int fp8_slot_expert(const Fp8Route& r, int i, bool& bad) {
+  const uint32_t q = static_cast<uint32_t>(i) / static_cast<uint32_t>(r.s);
+  const int64_t t = q, s = i - static_cast<int>(q) * r.s;
+  if (r.compute && !r.compute[t * r.compute_stride + s]) return -1;
+  const int64_t e = r.sel[t * r.sel_stride + s];
+  if (e < 0 || e >= r.e) {
+    bad = true;
+    return -1;
+  }
+  return static_cast<int>(e);
+}
+
+constexpr int kFp8PlanThreads = 1024;
+constexpr int kFp8MaxExperts = 2048;
+
+// One CTA: counts per expert, first position of each expert's slots, the slots in that order
+// (any order within an expert: a row's result does not depend on its place), and the groups
+// of at most group_rows rows of one expert: groups[i] = (expert, first position, rows, 0).
+__global__ void __launch_bounds__(kFp8PlanThreads) k_fp8_plan(Fp8Route r, int group_rows, int* sorted, int4* groups,
+                                                             int* n_groups) {
+  extern __shared__ int plan_smem[];
+  int* count = plan_smem;        // [E], then the next free position
+  int* first = plan_smem + r.e;  // [E]
+  __shared__ int s_warp[32][2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int n = r.q * r.s;
+  for (int e = tid; e < r.e; e += kFp8PlanThreads) count[e] = 0;
+  __syncthreads();
+  bool bad = false;
+  for (int i = tid; i < n; i += kFp8PlanThreads) {
+    const int e = fp8_slot_expert(r, i, bad);
+    if (e >= 0) atomicAdd(&count[e], 1);
+  }
+  if (bad && r.err) atomicOr(r.err, static_cast<uint32_t>(kErrBadExpert));
+  __syncthreads();
+  // Exclusive prefix of (slots, groups) over the experts, two consecutive experts per thread.
+  int c[2], g[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int e = 2 * tid + j;
+    c[j] = e < r.e ? count[e] : 0;
+    g[j] = (c[j] + group_rows - 1) / group_rows;
+  }
+  int sc = c[0] + c[1], sg = g[0] + g[1];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int pc = __shfl_up_sync(0xffffffffu, sc, o), pg = __shfl_up_sync(0xffffffffu, sg, o);
+    if (lane >= o) {
+      sc += pc;
+      sg += pg;
+    }
+  }
+  if (lane == 31) {
+    s_warp[warp][0] = sc;
+    s_warp[warp][1] = sg;
+  }
+  __syncthreads();
+  int bc = 0, bg = 0;
+  for (int w = 0; w < warp; ++w) {
+    bc += s_warp[w][0];
+    bg += s_warp[w][1];
+  }
+  int pos = bc + sc - c[0] - c[1], gi = bg + sg - g[0] - g[1];
+  if (tid == kFp8PlanThreads - 1) *n_groups = bg + sg;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int e = 2 * tid + j;
+    if (e < r.e) {
+      first[e] = pos;
+      for (int k = 0; k < g[j]; ++k)
+        groups[gi + k] = make_int4(e, pos + k * group_rows, min(group_rows, c[j] - k * group_rows), 0);
+    }
+    pos += c[j];
+    gi += g[j];
+  }
+  __syncthreads();
+  for (int e = tid; e < r.e; e += kFp8PlanThreads) count[e] = first[e];
+  __syncthreads();
+  for (int i = tid; i < n; i += kFp8PlanThreads) {
+    const int e = fp8_slot_expert(r, i, bad);
+    if (e >= 0) sorted[atomicAdd(&count[e], 1)] = i;
+  }
+}
+
+// ---- the weight-streaming product ---------------------------------------------------------------
+//
+// For few rows per weight the time is the weights' way from HBM. A CTA takes 8 rows of x (the
+// N of mma.sync m16n8k32, weights as the M operand) and 32 weight rows: two 16-row tiles,
+// which are the gate and the up rows of 16 hidden units, or 32 adjacent output columns. Its
+// warps split K by blocks of 128 and add up through shared memory in warp order. Every
+// operand goes from global memory straight to registers: a lane reads 16 consecutive bytes of
+// its weight row (4 lanes a row, both 64-byte halves of a block), and since a dot product may
+// be taken in any order of k, those words are used as they come, x's in the same order; no
+// shared memory, no shuffle. x is quantised in registers by the warp that needs it: lane
+// (g, c) holds 32 of row g's 128 columns, four lanes agree on the maximum.
+// The slots of an expert are served 8 at a time; a group's first slot leads (no plan pass).
+
+constexpr int kStreamRows = 8;        // rows of x per CTA
+constexpr int kStreamWRows = 16;      // weight rows per tile, two tiles per CTA
+constexpr int kStreamMaxWarps = 8;
+constexpr int kStreamMaxSlots = 512;  // slots a leader search looks through
+
+enum Fp8Mode { kFp8Linear = 0, kFp8GateUp = 1, kFp8Down = 2 };
+
+struct StreamArgs {
+  Fp8Route r;               // GateUp, Down
+  const int* sorted;        // GateUp, Down: planned groups (NULL: leaders)
+  const int4* groups;
+  const int* n_groups;
+  const void* x;            // rows of x: m rows (Linear), q tokens (GateUp), slots (Down, fp32)
+  int64_t x_stride;
+  int x_vec;                // rows can be read 16 bytes at a time
+  int m, n, k;              // rows (Linear), weight rows (per half), reduction length
+  const uint8_t* w;         // row r of expert e: w + e * w_stride_e + r * w_stride
+  int64_t w_stride, w_stride_e, w_stride_half;
+  const float* ws;          // scales, contiguous [E][halves][blocks n][blocks k]
+  void* out;                // Linear: [m, n]; GateUp: fp32 [slots][n]; Down: [q, s, n]
+  int out_dtype;
+  int64_t out_stride, out_stride_s;
+  int zero_skipped;
+};
+
+__device__ __forceinline__ uint4 ldg_stream(const uint8_t* p) {  // read once: past L1
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+// 16 bytes of a weight row from column c on, zero from column k on.
+__device__ __forceinline__ uint4 weight16(const uint8_t* row, int c, int k, bool live) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (live && c < k) {
+    v = ldg_stream(row + c);
+    if (c + 16 > k) {  // the row's last chunk: what pads the row is no data
+      uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int have = k - c - 4 * j;
+        if (have <= 0) w[j] = 0;
+        else if (have < 4) w[j] &= (1u << (8 * have)) - 1u;
+      }
+    }
+  }
+  return v;
+}
+// 16 elements of a row of x from column c on, zero from column k on.
+// COHERENT: the rows were written by the kernel this one may overlap (not the read-only path).
+template <typename TX, bool COHERENT>
+__device__ __forceinline__ void x16(const TX* row, int c, int k, bool live, bool vec, float (&v)[16]) {
+  if (live && vec && c + 16 <= k) {
+    if constexpr (COHERENT) {
+      static_assert(sizeof(TX) == 4, "fp32 rows");
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4 f = __ldcg(reinterpret_cast<const float4*>(row + c) + j);
+        v[4 * j] = f.x;
+        v[4 * j + 1] = f.y;
+        v[4 * j + 2] = f.z;
+        v[4 * j + 3] = f.w;
+      }
+      return;
+    }
+    float (&lo)[8] = reinterpret_cast<float (&)[8]>(v[0]);
+    float (&hi)[8] = reinterpret_cast<float (&)[8]>(v[8]);
+    load8<TX>(row + c, lo);
+    load8<TX>(row + c + 8, hi);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] = live && c + j < k ? to_f32<TX>(COHERENT ? __ldcg(row + c + j) : row[c + j]) : 0.f;
+}
+__device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+
+template <typename TX, int MODE>
+__global__ void __launch_bounds__(32 * kStreamMaxWarps) k_fp8_stream(StreamArgs a) {
+  constexpr unsigned kAll = 0xffffffffu;
+  __shared__ float red[kStreamMaxWarps][2][kStreamRows][kStreamWRows + 1];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nwarps = blockDim.x >> 5;
+  const int g = lane >> 2, c = lane & 3;
+  const int y = blockIdx.x;  // rows: CTAs that share weights run together
+  const int slice = blockIdx.y;
+  pdl_launch_dependents();
+  // This CTA's rows: lane m < cnt holds the m-th (Linear: row, otherwise slot).
+  int cnt, member = 0, expert = 0;
+  if constexpr (MODE == kFp8Linear) {
+    cnt = min(kStreamRows, a.m - y * kStreamRows);
+    member = y * kStreamRows + lane;
+  } else if (a.groups) {
+    if (y >= *a.n_groups) return;
+    const int4 gr = a.groups[y];
+    expert = gr.x;
+    cnt = gr.z;
+    if (lane < cnt) member = a.sorted[gr.y + lane];
+  } else {
+    bool bad = false;
+    const int mine = fp8_slot_expert(a.r, y, bad);
+    if (bad && a.r.err && tid == 0 && slice == 0) atomicOr(a.r.err, static_cast<uint32_t>(kErrBadExpert));
+    if (mine < 0) {
+      if (MODE == kFp8Down && a.zero_skipped) {
+        const int64_t o = static_cast<int64_t>(y / a.r.s) * a.out_stride + (y % a.r.s) * a.out_stride_s;
+        for (int i = tid; i < 2 * kStreamWRows; i += blockDim.x) {
+          const int col = slice * 2 * kStreamWRows + i;
+          if (col < a.n) store_any(a.out, o + col, 0.f, a.out_dtype);
+        }
+      }
+      return;
+    }
+    expert = mine;
+    const int n = a.r.q * a.r.s;
+    int before = 0;
+    cnt = 0;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      bool ignored = false;
+      const bool same = i0 + lane < n && fp8_slot_expert(a.r, i0 + lane, ignored) == mine;
+      unsigned hits = __ballot_sync(kAll, same);
+      if (i0 <= y) {
+        const unsigned below = y - i0 < 32 ? (1u << (y - i0)) - 1u : kAll;
+        before += __popc(hits & below);
+        hits &= ~below;
+      }
+      while (hits && cnt < kStreamRows) {
+        const int b = __ffs(hits) - 1;
+        hits &= hits - 1;
+        if (lane == cnt) member = i0 + b;
+        ++cnt;
+      }
+    }
+    if (before % kStreamRows) return;
+  }
+  const int r0 = slice * (MODE == kFp8GateUp ? kStreamWRows : 2 * kStreamWRows);
+  const int kblocks = fp8_blocks(a.k), nblocks = fp8_blocks(a.n);
+  const uint8_t* wrow[2];
+  const float* wscale[2];
+  bool lo_live[2], hi_live[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = r0 + (MODE == kFp8GateUp ? 0 : i * kStreamWRows);
+    const int half = MODE == kFp8GateUp ? i : 0;
+    wrow[i] = a.w + expert * a.w_stride_e + half * a.w_stride_half + static_cast<int64_t>(row + g) * a.w_stride;
+    wscale[i] = a.ws + ((static_cast<int64_t>(expert) * (MODE == kFp8GateUp ? 2 : 1) + half) * nblocks +
+                        min(row / kFp8Block, nblocks - 1)) * kblocks;
+    lo_live[i] = row + g < a.n;
+    hi_live[i] = row + g + 8 < a.n;
+  }
+  const int src = __shfl_sync(kAll, member, g);
+  const TX* xrow = static_cast<const TX*>(a.x) + static_cast<int64_t>(MODE == kFp8GateUp ? src / a.r.s : src) * a.x_stride;
+  const bool live = g < cnt;
+  float acc[2][4] = {};
+  bool waited = false;
+  for (int kb = warp; kb < kblocks; kb += nwarps) {
+    uint4 wv[2][2][2];  // [tile][half row][64-byte half]
+    const int c0 = kb * kFp8Block + 16 * c;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        wv[i][0][j] = weight16(wrow[i], c0 + 64 * j, a.k, lo_live[i]);
+        wv[i][1][j] = weight16(wrow[i] + 8 * a.w_stride, c0 + 64 * j, a.k, hi_live[i]);
+      }
+    const float sw0 = wscale[0][kb], sw1 = wscale[1][kb];
+    if (MODE == kFp8Down && !waited) pdl_wait();  // the weights are on their way meanwhile
+    waited = true;
+    float xv[2][16];
+    x16<TX, MODE == kFp8Down>(xrow, c0, a.k, live, a.x_vec, xv[0]);
+    x16<TX, MODE == kFp8Down>(xrow, c0 + 64, a.k, live, a.x_vec, xv[1]);
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) m = max(m, max(abs_bits(xv[0][j]), abs_bits(xv[1][j])));
+    m = max(m, __shfl_xor_sync(kAll, m, 1));
+    m = max(m, __shfl_xor_sync(kAll, m, 2));
+    const float am = fp8_amax(m);
+    const float f = kE4m3Max / am, sx = am / kE4m3Max;
+    const float sx0 = __shfl_sync(kAll, sx, 8 * c), sx1 = __shfl_sync(kAll, sx, 8 * c + 4);
+    float d[2][4] = {};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint32_t xq[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        xq[i] = e4m3x4(xv[j][4 * i] * f, xv[j][4 * i + 1] * f, xv[j][4 * i + 2] * f, xv[j][4 * i + 3] * f);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        mma_e4m3(d[i], wv[i][0][j].x, wv[i][1][j].x, wv[i][0][j].y, wv[i][1][j].y, xq[0], xq[1]);
+        mma_e4m3(d[i], wv[i][0][j].z, wv[i][1][j].z, wv[i][0][j].w, wv[i][1][j].w, xq[2], xq[3]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float sw = i ? sw1 : sw0;
+      acc[i][0] = fmaf(d[i][0], sx0 * sw, acc[i][0]);
+      acc[i][1] = fmaf(d[i][1], sx1 * sw, acc[i][1]);
+      acc[i][2] = fmaf(d[i][2], sx0 * sw, acc[i][2]);
+      acc[i][3] = fmaf(d[i][3], sx1 * sw, acc[i][3]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    red[warp][i][2 * c][g] = acc[i][0];
+    red[warp][i][2 * c + 1][g] = acc[i][1];
+    red[warp][i][2 * c][g + 8] = acc[i][2];
+    red[warp][i][2 * c + 1][g + 8] = acc[i][3];
+  }
+  __syncthreads();
+  // Sums over the warps, 16 consecutive columns of a row by 16 consecutive threads. A warp
+  // handles whole rows, so that the member comes by a shuffle.
+  const int per = MODE == kFp8GateUp ? kStreamRows * kStreamWRows : 2 * kStreamRows * kStreamWRows;
+  for (int o = tid; o < per; o += blockDim.x) {  // per and blockDim.x are multiples of 32
+    const int col = o & 15, row = (o >> 4) & 7, i = o >> 7;
+    float v = 0.f, u = 0.f;
+    for (int w = 0; w < nwarps; ++w) {
+      v += red[w][MODE == kFp8GateUp ? 0 : i][row][col];
+      if (MODE == kFp8GateUp) u += red[w][1][row][col];
+    }
+    const int dst = __shfl_sync(kAll, member, row);
+    const int wr = r0 + (MODE == kFp8GateUp ? 0 : i * kStreamWRows) + col;
+    if (row >= cnt || wr >= a.n) continue;
+    if constexpr (MODE == kFp8GateUp) {
+      static_cast<float*>(a.out)[static_cast<int64_t>(dst) * a.out_stride + wr] = silu_mul(v, u);
+    } else if constexpr (MODE == kFp8Down) {
+      store_any(a.out, static_cast<int64_t>(dst / a.r.s) * a.out_stride + (dst % a.r.s) * a.out_stride_s + wr, v, a.out_dtype);
+    } else {
+      store_any(a.out, static_cast<int64_t>(dst) * a.out_stride + wr, v, a.out_dtype);
+    }
+  }
+}
+
+// Rows of slots that are not computed, set to zero (planned batches).
+__global__ void __launch_bounds__(256) k_fp8_zero_skipped(Fp8Route r, int h, void* out, int dtype, int64_t stride_t,
+                                                         int64_t stride_s) {
+  const int n = r.q * r.s;
+  for (int i = blockIdx.x; i < n; i += gridDim.x) {
+    bool bad = false;
+    if (fp8_slot_expert(r, i, bad) >= 0) continue;
+    const int64_t o = static_cast<int64_t>(i / r.s) * stride_t + (i % r.s) * stride_s;
+    for (int j = threadIdx.x; j < h; j += blockDim.x) store_any(out, o + j, 0.f, dtype);
+  }
+}
+
+}  // namespace alut

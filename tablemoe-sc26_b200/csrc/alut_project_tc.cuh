@@ -131,15 +131,6 @@ inline bool pt_encode_x_map(CUtensorMap* map, const void* x, int64_t q, int64_t 
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// 2D TMA tile load (no multicast): box at (x = column, y = row) of the map into smem.
-__device__ __forceinline__ void pt_tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
-          "r"(smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_addr(bar))
-      : "memory");
-}
-
 // kind::f16 instruction descriptor: fp32 D, bf16 A and B, K-major, M = 128, N = n.
 __host__ __device__ __forceinline__ uint32_t pt_idesc(int n) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
@@ -151,17 +142,6 @@ __device__ __forceinline__ uint64_t pt_desc(uint32_t saddr, uint32_t lbo, uint32
   d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFF) << 16;
   d |= static_cast<uint64_t>((sbo >> 4) & 0x3FFF) << 32;
   d |= static_cast<uint64_t>(1) << 46;
-  return d;
-}
-// K-major operand with the 128-byte swizzle: 8-row atoms of 1 KB (SBO), rows of 128 B;
-// within an atom the K offset is added to the start address.
-__device__ __forceinline__ uint64_t pt_desc_sw128(uint32_t saddr) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFF);
-  d |= static_cast<uint64_t>(1) << 16;           // LBO (unused for swizzled K-major)
-  d |= static_cast<uint64_t>(1024 >> 4) << 32;   // SBO: next 8-row atom
-  d |= static_cast<uint64_t>(1) << 46;           // descriptor version
-  d |= static_cast<uint64_t>(2) << 61;           // layout: 128-byte swizzle
   return d;
 }
 __device__ __forceinline__ void pt_mma(uint32_t tmem, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {

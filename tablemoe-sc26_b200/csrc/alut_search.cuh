@@ -14,6 +14,7 @@
 #pragma once
 
 #include "alut_common.cuh"
+#include "alut_ptx.cuh"
 
 namespace alut {
 
@@ -30,7 +31,6 @@ struct SearchArgs {
 };
 
 constexpr int kTmaBuffers = 2;
-constexpr uint32_t kWaitLimit = 1u << 20;  // bounded mbarrier wait (iterations of try_wait)
 constexpr int kBatch = 4;                   // slots scored together per pass over a row
 constexpr int kDecodeMaxPairs = 256;
 constexpr int kDecodeMaxTokens = kDecodeMaxPairs;  // any batch of <= 256 slots
@@ -39,54 +39,6 @@ constexpr int kDecodeMaxTokens = kDecodeMaxPairs;  // any batch of <= 256 slots
 #endif
 constexpr int kDecodeRun = ALUT_DECODE_RUN;  // slots of one table a decode-scan leader serves
 static_assert(kDecodeRun <= kSearchGroup, "runs fit the scoring group");
-
-// ---- TMA / mbarrier primitives ---------------------------------------------------------
-
-__device__ __forceinline__ uint32_t smem_addr(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes)
-               : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(smem_addr(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ uint64_t global_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-// Wait with a deadline of kWaitNs (each try_wait may itself suspend for a while, so the
-// bound is on time, not on the number of tries); false if the deadline passed.
-constexpr uint64_t kWaitNs = 1000000000ull;  // 1 s
-__device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity) {
-  const uint64_t t0 = global_ns();
-  for (uint32_t n = 0; n < kWaitLimit; ++n) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if (global_ns() - t0 > kWaitNs) return false;
-  }
-  return false;
-}
-__device__ __forceinline__ void bulk_g2s(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          smem_addr(dst)),
-      "l"(src), "r"(bytes), "r"(smem_addr(bar))
-      : "memory");
-}
-__device__ __forceinline__ void fence_async_shared() {
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
 
 // Rows land in shared memory with a 16-byte pad after each (pitch = L*esz + 16): the 8
 // threads of a shared-memory phase, reading the same 16-byte unit of 8 consecutive rows,

@@ -60,6 +60,22 @@ class SearchParams(ctypes.Structure):
     ]
 
 
+class Router(ctypes.Structure):
+    _fields_ = [
+        ("num_experts", ctypes.c_int32), ("top_k", ctypes.c_int32), ("scoring", ctypes.c_int32),
+        ("n_group", ctypes.c_int32), ("topk_group", ctypes.c_int32), ("group_rule", ctypes.c_int32),
+        ("normalize_topk", ctypes.c_int32), ("scale", ctypes.c_float), ("bias", ctypes.c_void_p),
+    ]
+
+
+class Fp8ExpertWeights(ctypes.Structure):
+    _fields_ = [
+        ("num_experts", ctypes.c_int32), ("h", ctypes.c_int32), ("i", ctypes.c_int32), ("reserved0", ctypes.c_int32),
+        ("gate_up", ctypes.c_void_p), ("gate_up_stride", ctypes.c_int64 * 3), ("gate_up_scale", ctypes.c_void_p),
+        ("down", ctypes.c_void_p), ("down_stride", ctypes.c_int64 * 2), ("down_scale", ctypes.c_void_p),
+    ]
+
+
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
@@ -67,6 +83,8 @@ _SZ = ctypes.c_size_t
 _TP = ctypes.POINTER(Tables)
 _BP = ctypes.POINTER(Batch)
 _PP = ctypes.POINTER(SearchParams)
+_RP = ctypes.POINTER(Router)
+_EP = ctypes.POINTER(Fp8ExpertWeights)
 
 SIGNATURES = {
     "alut_workspace_size": (_SZ, [_TP, _I32, _I32]),
@@ -100,6 +118,15 @@ SIGNATURES = {
                                   _P, _I64, _P, _SZ, _P]),
     "alut_keep_mask": (ctypes.c_int, [_I32, _I32, _I32, _P, _P, _I64, _P, ctypes.c_double, _P, _P, _I64, _P, _SZ,
                                       _P]),
+    "alut_route_experts": (ctypes.c_int, [_RP, _I32, _P, _I32, _I64, _I32, _I32, ctypes.c_double, _P, _P, _P, _P, _P,
+                                          _I64, _P, _SZ, _P]),
+    "alut_quantize_fp8": (ctypes.c_int, [_I64, _I64, _I32, _I32, _P, _I32, _I64, _I64, _P, _I64, _I64, _P, _P]),
+    "alut_linear_fp8_workspace_size": (_SZ, [_I32, _I32, _I32]),
+    "alut_linear_fp8": (ctypes.c_int, [_I32, _I32, _I32, _P, _I32, _I64, _P, _I64, _P, _P, _I32, _I64, _P, _P, _SZ,
+                                       _P]),
+    "alut_experts_fp8_workspace_size": (_SZ, [_EP, _I32, _I32]),
+    "alut_experts_fp8": (ctypes.c_int, [_EP, _I32, _I32, _P, _I32, _I64, _P, _I64, _P, _I64, _I32, _P, _I32, _I64,
+                                        _I64, _P, _P, _SZ, _P]),
     "alut_normalize_rows": (ctypes.c_int, [_I64, _I32, _P, _I64, _P, _I64, _I32, ctypes.c_float, _P]),
     "alut_workspace_errors": (ctypes.c_int, [_P, _SZ, _I32, ctypes.POINTER(ctypes.c_uint32), _P]),
     "alut_set_profile_events": (ctypes.c_int, [_P, _P]),

@@ -1,0 +1,210 @@
+"""Products in 8-bit floating point (e4m3) with a scale for each block of 128, on the
+``alut_quantize_fp8``, ``alut_linear_fp8`` and ``alut_experts_fp8`` kernels of ``libalut.so``.
+
+New: the reference computes the experts that are not looked up in a Python loop over the
+routed experts (``qwen3_vl_moe/cached_layers.py:431-437``). ``Fp8Experts`` is that loop as one
+call, with the signature of ``ALUTCachedMoE``'s ``run_experts``; ``Fp8Linear`` is the plain
+product (shared experts, projections). Weights hold one fp32 scale per 128 x 128 block;
+activations are taken in their 8-bit form inside the call, one scale per row and 128 columns.
+Inference only; there is no torch fallback: CUDA tensors are required.
+"""
+from __future__ import annotations
+
+import torch
+
+from ..cache_engine import _alut
+from ..cache_engine.config import CacheConfig
+
+BLOCK = 128
+_E4M3 = torch.float8_e4m3fn
+
+
+def _blocks(n):
+    return -(-n // BLOCK)
+
+
+def quantize_fp8(x, block_rows=1):
+    """(e4m3 [..., rows, cols], fp32 scales [..., ceil(rows / block_rows), ceil(cols / 128)]) of x
+    (f32, bf16 or f16; at least 2D): block_rows 1 for activations, 128 for weights."""
+    if x.device.type != "cuda":
+        raise ValueError("quantize_fp8: CUDA tensors only")
+    if x.dim() < 2:
+        raise ValueError(f"quantize_fp8 expects at least 2 dimensions, got {tuple(x.shape)}")
+    if block_rows not in (1, BLOCK):
+        raise ValueError(f"block_rows must be 1 or {BLOCK}, got {block_rows}")
+    lead, (rows, cols) = x.shape[:-2], x.shape[-2:]
+    code = _alut.dtype_code(x.dtype)
+    v = x if x.dim() == 2 and x.stride(-1) == 1 and x.stride(0) >= cols else x.contiguous()
+    q = torch.empty(x.shape, dtype=_E4M3, device=x.device)
+    s = torch.empty(*lead, -(-rows // block_rows), _blocks(cols), dtype=torch.float32, device=x.device)
+    batch = lead.numel()
+    stride = v.stride(0) if v.dim() == 2 else cols
+    rc = _alut.load().alut_quantize_fp8(batch, rows, cols, block_rows, v.data_ptr(), code, rows * cols, max(stride, cols),
+                                        q.data_ptr(), rows * cols, cols, s.data_ptr(), _alut.stream_ptr(x.device))
+    _alut.check(rc, "alut_quantize_fp8")
+    return q, s
+
+
+def _padded(w):
+    """w (e4m3 [..., n, k]) with rows that start on 16 bytes: itself where it is so already."""
+    k = w.shape[-1]
+    ok = w.stride(-1) == 1 and w.stride(-2) >= -(-k // 16) * 16 and all(s % 16 == 0 for s in w.stride()[:-1])
+    if ok and w.data_ptr() % 16 == 0:
+        return w
+    out = torch.zeros(*w.shape[:-1], -(-k // 16) * 16, dtype=torch.uint8, device=w.device)
+    out[..., :k] = w.view(torch.uint8)
+    return out.view(_E4M3)[..., :k]
+
+
+def _check_weight(w, scale, name, dims):
+    if w.dtype != _E4M3:
+        raise ValueError(f"{name} must be torch.float8_e4m3fn, got {w.dtype}")
+    if w.device.type != "cuda":
+        raise ValueError(f"{name} must be a CUDA tensor (the 8-bit products have no CPU path)")
+    if w.dim() != dims or 0 in w.shape:
+        raise ValueError(f"{name} must be a non-empty {dims}D tensor, got {tuple(w.shape)}")
+    want = (*w.shape[:-2], _blocks(w.shape[-2]), _blocks(w.shape[-1]))
+    if tuple(scale.shape) != want or scale.dtype != torch.float32 or scale.device != w.device:
+        raise ValueError(f"{name}'s scales must be fp32 {want} on {w.device}, got {scale.dtype} {tuple(scale.shape)}")
+
+
+class _Fp8Module:
+    def _init_device(self, device):
+        self.device = device
+        self._lib = _alut.load()
+        self._errors = torch.zeros(1, dtype=torch.int32, device=device)
+
+    def _check_x(self, x, width):
+        if x.device != self.device:
+            raise ValueError(f"x is on {x.device}, the weights on {self.device}")
+        if x.dim() < 1 or x.shape[-1] != width:
+            raise ValueError(f"x must have {width} columns, got {tuple(x.shape)}")
+        x = x.reshape(-1, width)
+        if x.stride(-1) != 1 or x.stride(0) < width:  # also a broadcast row
+            x = x.contiguous()
+        return x, _alut.dtype_code(x.dtype)
+
+    def _row_stride(self, x):
+        return max(x.stride(0), x.shape[-1])
+
+    def device_errors(self, clear=True):
+        """Error bits (ALUT_ERR_*) that this object's calls have set; waits for the current stream."""
+        bits = int(self._errors.item())
+        if clear and bits:
+            self._errors.zero_()
+        return bits
+
+    def _finish(self, what):
+        if CacheConfig.ALUT_CHECK_ERRORS:
+            _alut.raise_device_errors(self.device_errors(), what)
+
+
+class Fp8Linear(_Fp8Module):
+    """y = x W^T with W e4m3 [N, K] and its fp32 block scales [ceil(N/128), ceil(K/128)].
+
+    The weights are kept as given when K % 16 == 0 and they are contiguous; otherwise one
+    padded copy is made here."""
+
+    def __init__(self, weight, scale):
+        _check_weight(weight, scale, "weight", 2)
+        self._init_device(weight.device)
+        self.n, self.k = weight.shape
+        self.weight, self.scale = _padded(weight), scale.contiguous()
+
+    @classmethod
+    def quantize(cls, weight):
+        """From a weight [N, K] in f32, bf16 or f16."""
+        return cls(*quantize_fp8(weight, BLOCK))
+
+    def __call__(self, x, out=None, *, out_dtype=None):
+        """x [..., K] (f32, bf16 or f16) -> [..., N] in ``out_dtype`` (default x's), or into ``out``
+        (a 2D tensor [rows, N] with unit innermost stride)."""
+        v, xd = self._check_x(x, self.k)
+        m = v.shape[0]
+        if out is None:
+            y = torch.empty(*x.shape[:-1], self.n, dtype=out_dtype or x.dtype, device=x.device)
+            stride = self.n
+        else:
+            if out.shape != (m, self.n) or out.device != x.device or out.stride(-1) != 1:
+                raise ValueError(f"out must be a [{m}, {self.n}] tensor on {x.device} with unit innermost stride")
+            if out_dtype is not None and out_dtype != out.dtype:
+                raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
+            y, stride = out, out.stride(0) if m > 1 else max(out.stride(0), self.n)
+        n = int(self._lib.alut_linear_fp8_workspace_size(m, self.n, self.k))
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+        rc = self._lib.alut_linear_fp8(m, self.n, self.k, v.data_ptr(), xd, self._row_stride(v), self.weight.data_ptr(),
+                                       self.weight.stride(0), self.scale.data_ptr(), y.data_ptr(),
+                                       _alut.dtype_code(y.dtype), stride, self._errors.data_ptr(), ws.data_ptr(), n,
+                                       _alut.stream_ptr(x.device))
+        _alut.check(rc, "alut_linear_fp8")
+        self._finish("alut_linear_fp8")
+        return y
+
+
+class Fp8Experts(_Fp8Module):
+    """The routed experts of a layer, down(silu(gate x) * (up x)).
+
+    ``gate_up`` e4m3 [E, 2, I, H] (gate rows, then up rows) with scales [E, 2, ceil(I/128),
+    ceil(H/128)]; ``down`` e4m3 [E, H, I] with scales [E, ceil(H/128), ceil(I/128)]. Kept as given
+    when H and I are multiples of 16 and they are contiguous; otherwise one padded copy."""
+
+    def __init__(self, gate_up, gate_up_scale, down, down_scale):
+        _check_weight(gate_up, gate_up_scale, "gate_up", 4)
+        _check_weight(down, down_scale, "down", 3)
+        e, two, i, h = gate_up.shape
+        if two != 2 or tuple(down.shape) != (e, h, i) or down.device != gate_up.device:
+            raise ValueError(f"gate_up [E, 2, I, H] and down [E, H, I] do not fit: {tuple(gate_up.shape)}, "
+                             f"{tuple(down.shape)}")
+        self._init_device(gate_up.device)
+        self.num_experts, self.inner, self.hidden = e, i, h
+        self.gate_up, self.down = _padded(gate_up), _padded(down)
+        self.gate_up_scale, self.down_scale = gate_up_scale.contiguous(), down_scale.contiguous()
+        w = _alut.Fp8ExpertWeights()
+        w.num_experts, w.h, w.i = e, h, i
+        w.gate_up, w.gate_up_scale = self.gate_up.data_ptr(), self.gate_up_scale.data_ptr()
+        w.gate_up_stride[:] = list(self.gate_up.stride()[:3])
+        w.down, w.down_scale = self.down.data_ptr(), self.down_scale.data_ptr()
+        w.down_stride[:] = list(self.down.stride()[:2])
+        self._weights = w
+
+    @classmethod
+    def quantize(cls, gate_up, down):
+        """From weights [E, 2, I, H] and [E, H, I] in f32, bf16 or f16."""
+        return cls(*quantize_fp8(gate_up, BLOCK), *quantize_fp8(down, BLOCK))
+
+    def __call__(self, x, selected_experts, compute_mask=None, collected=None):
+        """Outputs [Q, S, H] of the experts ``selected_experts`` [Q, S] on the tokens x [Q, H], for
+        the slots of ``compute_mask`` [Q, S] (None: all). Without ``collected`` a new tensor of x's
+        dtype, 0 at the other slots; otherwise written into it (f32, bf16 or f16, unit innermost
+        stride), its other rows untouched: the form of ``ALUTCachedMoE``'s ``run_experts``."""
+        v, xd = self._check_x(x, self.hidden)
+        if selected_experts.dim() != 2 or selected_experts.shape[0] != v.shape[0]:
+            raise ValueError(f"selected_experts must be [{v.shape[0]}, S], got {tuple(selected_experts.shape)}")
+        if selected_experts.dtype != torch.int64 or selected_experts.device != x.device:
+            raise ValueError("selected_experts must be int64 on x's device")
+        q, s = selected_experts.shape
+        sel = selected_experts if selected_experts.stride(-1) == 1 else selected_experts.contiguous()
+        comp = None
+        if compute_mask is not None:
+            if compute_mask.shape != (q, s) or compute_mask.dtype not in (torch.bool, torch.uint8) \
+                    or compute_mask.device != x.device:
+                raise ValueError(f"compute_mask must be bool [{q}, {s}] on x's device")
+            comp = compute_mask if compute_mask.stride(-1) == 1 and compute_mask.stride(0) >= s \
+                else compute_mask.contiguous()
+        if sel.stride(0) < s:
+            sel = sel.contiguous()
+        out = collected
+        if out is None:
+            out = torch.empty(q, s, self.hidden, dtype=x.dtype, device=x.device)
+        elif out.shape != (q, s, self.hidden) or out.device != x.device or out.stride(-1) != 1:
+            raise ValueError(f"collected must be [{q}, {s}, {self.hidden}] on {x.device} with unit innermost stride")
+        n = int(self._lib.alut_experts_fp8_workspace_size(self._weights, q, s))
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+        rc = self._lib.alut_experts_fp8(self._weights, q, s, v.data_ptr(), xd, self._row_stride(v), sel.data_ptr(),
+                                        max(sel.stride(0), s), _alut.ptr(comp), s if comp is None else max(comp.stride(0), s),
+                                        int(collected is None), out.data_ptr(), _alut.dtype_code(out.dtype), out.stride(0),
+                                        out.stride(1), self._errors.data_ptr(), ws.data_ptr(), n,
+                                        _alut.stream_ptr(x.device))
+        _alut.check(rc, "alut_experts_fp8")
+        self._finish("alut_experts_fp8")
+        return out
