@@ -248,9 +248,6 @@ enum Fp8Mode { kFp8Linear = 0, kFp8GateUp = 1, kFp8Down = 2 };
 
 struct StreamArgs {
   Fp8Route r;               // GateUp, Down
-  const int* sorted;        // GateUp, Down: planned groups (NULL: leaders)
-  const int4* groups;
-  const int* n_groups;
   const void* x;            // rows of x: m rows (Linear), q tokens (GateUp), slots (Down, fp32)
   int64_t x_stride;
   int x_vec;                // rows can be read 16 bytes at a time
@@ -337,12 +334,6 @@ __global__ void __launch_bounds__(32 * kStreamMaxWarps) k_fp8_stream(StreamArgs 
   if constexpr (MODE == kFp8Linear) {
     cnt = min(kStreamRows, a.m - y * kStreamRows);
     member = y * kStreamRows + lane;
-  } else if (a.groups) {
-    if (y >= *a.n_groups) return;
-    const int4 gr = a.groups[y];
-    expert = gr.x;
-    cnt = gr.z;
-    if (lane < cnt) member = a.sorted[gr.y + lane];
   } else {
     bool bad = false;
     const int mine = fp8_slot_expert(a.r, y, bad);

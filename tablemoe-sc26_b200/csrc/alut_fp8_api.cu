@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "alut_fp8.cuh"
+#include "alut_fp8_tc.cuh"
 #include "alut_host.cuh"
 
 namespace alut {
@@ -46,20 +47,109 @@ static int launch_stream(const StreamArgs& a, int x_dtype, unsigned groups, bool
   return ALUT_OK;
 }
 
+// TMA map of a byte tensor of up to 4 dimensions (strides in bytes of dimensions 1..): boxes of
+// 128 bytes x box_rows rows with the 128-byte swizzle, out-of-range parts read as zeros.
+static int encode_map(CUtensorMap* map, const void* p, int nd, const uint64_t* dims, const uint64_t* strides,
+                      uint32_t box_rows) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static Encode encode = nullptr;
+  if (!encode) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult qr{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qr) != cudaSuccess ||
+        qr != cudaDriverEntryPointSuccess || !fn)
+      return fail(ALUT_ECUDA, "cuTensorMapEncodeTiled is not available");
+    encode = reinterpret_cast<Encode>(fn);
+  }
+  cuuint64_t d[4], st[3];
+  const cuuint32_t box[4] = {kFp8Block, box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
+  for (int i = 0; i < nd; ++i) d[i] = dims[i];
+  for (int i = 0; i + 1 < nd; ++i) st[i] = strides[i];
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, nd, const_cast<void*>(p), d, st, box, estr,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(ALUT_ECUDA, "cuTensorMapEncodeTiled: error %d", static_cast<int>(r));
+  return ALUT_OK;
+}
+
+// 8-bit rows [rows][f8_row_pitch(k)].
+static int encode_rows(CUtensorMap* map, const void* p, int64_t rows, int k, uint32_t box_rows) {
+  const uint64_t dims[2] = {static_cast<uint64_t>(f8_row_pitch(k)), static_cast<uint64_t>(rows)};
+  const uint64_t strides[1] = {static_cast<uint64_t>(f8_row_pitch(k))};
+  return encode_map(map, p, 2, dims, strides, box_rows);
+}
+
+// A weight [experts][halves][rows][k]; a dimension of extent 1 takes any stride.
+static int encode_weight(CUtensorMap* map, const void* p, int k, int rows, int halves, int experts, int64_t row_stride,
+                         int64_t half_stride, int64_t expert_stride) {
+  const uint64_t any = static_cast<uint64_t>(row_stride);
+  const uint64_t dims[4] = {static_cast<uint64_t>(k), static_cast<uint64_t>(rows), static_cast<uint64_t>(halves),
+                            static_cast<uint64_t>(experts)};
+  const uint64_t strides[3] = {static_cast<uint64_t>(row_stride), halves > 1 ? static_cast<uint64_t>(half_stride) : any,
+                               experts > 1 ? static_cast<uint64_t>(expert_stride) : any};
+  return encode_map(map, p, 4, dims, strides, kF8Rows);
+}
+
+template <int MODE>
+static int launch_tc(const CUtensorMap& xm, const CUtensorMap& wm, const F8Args& a, int64_t max_tiles, cudaStream_t st) {
+  auto kern = k_fp8_tc<MODE>;
+  const int rc = allow_smem(reinterpret_cast<const void*>(kern), kF8SmemBytes);
+  if (rc) return rc;
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(max_tiles, num_sms()));
+  const cudaError_t e = launch_pdl(kern, dim3(grid), dim3(kF8Threads), kF8SmemBytes, st, xm, wm, a);
+  if (e != cudaSuccess) return fail(ALUT_ECUDA, "k_fp8_tc: %s", cudaGetErrorString(e));
+  return ALUT_OK;
+}
+
+static int launch_rows(const F8PrepArgs& a, int x_dtype, cudaStream_t st) {
+  const int64_t n = static_cast<int64_t>(a.rows) * fp8_blocks(a.k);
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((n + 15) / 16, 8 * num_sms()));
+  auto kern = x_dtype == ALUT_BF16 ? k_fp8_rows<__nv_bfloat16> : x_dtype == ALUT_F16 ? k_fp8_rows<__half> : k_fp8_rows<float>;
+  kern<<<grid, 256, 0, st>>>(a);
+  return check_launch("k_fp8_rows");
+}
+
+// Which product a call takes: the weight-streaming one below these row counts.
+static bool linear_streams(int m) { return m <= 16; }
+static bool experts_stream(int64_t slots) { return slots <= kStreamMaxSlots; }
+
+struct LinearWorkspace {
+  size_t xq, sx, total;
+};
+static LinearWorkspace linear_layout(int m, int k) {
+  LinearWorkspace w{};
+  size_t off = 0;
+  if (!linear_streams(m)) {
+    w.xq = off; off = align256(off + static_cast<size_t>(m) * f8_row_pitch(k));
+    w.sx = off; off = align256(off + sizeof(float) * m * f8_scale_pitch(k));
+  }
+  w.total = off + 256;
+  return w;
+}
+
 // Workspace of alut_experts_fp8, in order; every part starts on 256 bytes.
 struct ExpertsWorkspace {
-  size_t n_groups, groups, sorted, hidden, total;
+  size_t n_groups, groups, sorted, xq, sx, hidden, hs, total;
   int64_t max_groups;
 };
 static ExpertsWorkspace experts_layout(const alut_fp8_experts_t* ex, int q, int s) {
   ExpertsWorkspace w{};
   const int64_t n = static_cast<int64_t>(q) * s;
-  w.max_groups = ceil_div(n, kStreamRows) + std::min<int64_t>(n, ex->num_experts);
   size_t off = 0;
-  w.n_groups = off; off = align256(off + sizeof(int));
-  w.groups = off;   off = align256(off + sizeof(int4) * w.max_groups);
-  w.sorted = off;   off = align256(off + sizeof(int) * n);
-  w.hidden = off;   off = align256(off + sizeof(float) * n * round_up(ex->i, 4));
+  if (experts_stream(n)) {
+    w.hidden = off; off = align256(off + sizeof(float) * n * round_up(ex->i, 4));
+  } else {
+    w.max_groups = ceil_div(n, kF8Rows) + std::min<int64_t>(n, ex->num_experts);
+    w.n_groups = off; off = align256(off + sizeof(int));
+    w.groups = off;   off = align256(off + sizeof(int4) * w.max_groups);
+    w.sorted = off;   off = align256(off + sizeof(int) * n);
+    w.xq = off;       off = align256(off + static_cast<size_t>(q) * f8_row_pitch(ex->h));
+    w.sx = off;       off = align256(off + sizeof(float) * q * f8_scale_pitch(ex->h));
+    w.hidden = off;   off = align256(off + static_cast<size_t>(n) * f8_row_pitch(ex->i));
+    w.hs = off;       off = align256(off + sizeof(float) * n * f8_scale_pitch(ex->i));
+  }
   w.total = off;
   return w;
 }
@@ -112,7 +202,7 @@ int alut_quantize_fp8(int64_t batch, int64_t rows, int32_t cols, int32_t block_r
 
 size_t alut_linear_fp8_workspace_size(int32_t m, int32_t n, int32_t k) {
   if (m < 0 || n <= 0 || k <= 0) return 0;
-  return 256;
+  return linear_layout(m, k).total;
 }
 
 int alut_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, int32_t x_dtype, int64_t x_stride, const void* w,
@@ -128,6 +218,31 @@ int alut_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, int32_t x_dt
   const size_t need = alut_linear_fp8_workspace_size(m, n, k);
   if (!workspace || workspace_bytes < need)
     return fail(ALUT_EWORKSPACE, "linear_fp8: workspace has %zu bytes, needs %zu", workspace_bytes, need);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (!linear_streams(m)) {
+    if (!aligned16(workspace)) return fail(ALUT_EWORKSPACE, "linear_fp8: workspace must be 16-byte aligned");
+    const LinearWorkspace ws = linear_layout(m, k);
+    char* base = static_cast<char*>(workspace);
+    F8PrepArgs p{x, x_stride, m, k, rows_vec(x, x_stride, x_dtype), reinterpret_cast<uint8_t*>(base + ws.xq),
+                 reinterpret_cast<float*>(base + ws.sx)};
+    CUtensorMap xm, wm;
+    rc = encode_rows(&xm, p.xq, m, k, kF8Rows);
+    if (!rc) rc = encode_weight(&wm, w, k, n, 1, 1, w_stride, 0, 0);
+    if (!rc) rc = launch_rows(p, x_dtype, st);
+    if (rc) return rc;
+    F8Args a{};
+    a.m = m;
+    a.n = n;
+    a.k = k;
+    a.sx = p.sx;
+    a.ws = w_scale;
+    a.out = out;
+    a.out_dtype = out_dtype;
+    a.out_stride = out_stride;
+    a.out_vec = rows_vec(out, out_stride, out_dtype);
+    a.err = error_bits;
+    return launch_tc<kFp8Linear>(xm, wm, a, static_cast<int64_t>(ceil_div(m, kF8Rows)) * ((fp8_blocks(n) + 1) / 2), st);
+  }
   StreamArgs a{};
   a.x = x;
   a.x_stride = x_stride;
@@ -141,8 +256,7 @@ int alut_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, int32_t x_dt
   a.out = out;
   a.out_dtype = out_dtype;
   a.out_stride = out_stride;
-  return launch_stream<kFp8Linear>(a, x_dtype, static_cast<unsigned>(ceil_div(m, kStreamRows)), false,
-                                   reinterpret_cast<cudaStream_t>(stream));
+  return launch_stream<kFp8Linear>(a, x_dtype, static_cast<unsigned>(ceil_div(m, kStreamRows)), false, st);
 }
 
 size_t alut_experts_fp8_workspace_size(const alut_fp8_experts_t* ex, int32_t q, int32_t s) {
@@ -175,17 +289,25 @@ int alut_experts_fp8(const alut_fp8_experts_t* ex, int32_t q, int32_t s, const v
   char* base = static_cast<char*>(workspace);
   const int n = q * s;
   Fp8Route r{q, s, ex->num_experts, sel, sel_stride, compute, compute_stride, error_bits};
-  StreamArgs a{};
-  a.r = r;
-  const bool planned = n > kStreamMaxSlots;
-  unsigned groups = static_cast<unsigned>(n);
-  if (planned) {
+  if (!experts_stream(n)) {
+    F8PrepArgs p{x, x_stride, q, ex->h, rows_vec(x, x_stride, x_dtype), reinterpret_cast<uint8_t*>(base + ws.xq),
+                 reinterpret_cast<float*>(base + ws.sx)};
+    uint8_t* hq = reinterpret_cast<uint8_t*>(base + ws.hidden);
+    CUtensorMap xm, gm, hm, dm;
+    rc = encode_rows(&xm, p.xq, q, ex->h, 1);  // gathered row by row
+    if (!rc) rc = encode_rows(&hm, hq, n, ex->i, kF8Rows);
+    if (!rc)
+      rc = encode_weight(&gm, ex->gate_up, ex->h, ex->i, 2, ex->num_experts, ex->gate_up_stride[2],
+                         ex->gate_up_stride[1], ex->gate_up_stride[0]);
+    if (!rc)
+      rc = encode_weight(&dm, ex->down, ex->i, ex->h, 1, ex->num_experts, ex->down_stride[1], 0, ex->down_stride[0]);
+    if (rc) return rc;
+    F8Args a{};
     a.sorted = reinterpret_cast<int*>(base + ws.sorted);
     a.groups = reinterpret_cast<int4*>(base + ws.groups);
     a.n_groups = reinterpret_cast<int*>(base + ws.n_groups);
-    groups = static_cast<unsigned>(ws.max_groups);
     k_fp8_plan<<<1, kFp8PlanThreads, 2 * sizeof(int) * ex->num_experts, st>>>(
-        r, kStreamRows, reinterpret_cast<int*>(base + ws.sorted), reinterpret_cast<int4*>(base + ws.groups),
+        r, kF8Rows, reinterpret_cast<int*>(base + ws.sorted), reinterpret_cast<int4*>(base + ws.groups),
         reinterpret_cast<int*>(base + ws.n_groups));
     rc = check_launch("k_fp8_plan");
     if (rc) return rc;
@@ -195,7 +317,32 @@ int alut_experts_fp8(const alut_fp8_experts_t* ex, int32_t q, int32_t s, const v
       rc = check_launch("k_fp8_zero_skipped");
       if (rc) return rc;
     }
+    rc = launch_rows(p, x_dtype, st);
+    if (rc) return rc;
+    a.s = s;
+    a.err = error_bits;
+    a.n = ex->i;
+    a.k = ex->h;
+    a.sx = p.sx;
+    a.ws = ex->gate_up_scale;
+    a.hq = hq;
+    a.hs = reinterpret_cast<float*>(base + ws.hs);
+    rc = launch_tc<kFp8GateUp>(xm, gm, a, ws.max_groups * fp8_blocks(ex->i), st);
+    if (rc) return rc;
+    a.n = ex->h;
+    a.k = ex->i;
+    a.sx = a.hs;
+    a.ws = ex->down_scale;
+    a.out = out;
+    a.out_dtype = out_dtype;
+    a.out_stride = out_stride_t;
+    a.out_stride_s = out_stride_s;
+    a.out_vec = rows_vec(out, out_stride_t, out_dtype) && rows_vec(out, out_stride_s, out_dtype);
+    return launch_tc<kFp8Down>(hm, dm, a, ws.max_groups * ((fp8_blocks(ex->h) + 1) / 2), st);
   }
+  StreamArgs a{};
+  a.r = r;
+  const unsigned groups = static_cast<unsigned>(n);
   const int64_t hs = round_up(ex->i, 4);
   a.x = x;
   a.x_stride = x_stride;
@@ -225,7 +372,7 @@ int alut_experts_fp8(const alut_fp8_experts_t* ex, int32_t q, int32_t s, const v
   a.out_dtype = out_dtype;
   a.out_stride = out_stride_t;
   a.out_stride_s = out_stride_s;
-  a.zero_skipped = zero_skipped && !planned;
+  a.zero_skipped = zero_skipped;
   return launch_stream<kFp8Down>(a, ALUT_F32, groups, true, st);
 }
 
