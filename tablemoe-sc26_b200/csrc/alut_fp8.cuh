@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(256) k_fp8_quantize_blocks(QuantArgs a) {
   }
 }
 
-// ---- plan: computed slots grouped by expert ---------------------------------------------------
+// ---- routed slots --------------------------------------------------------------------------------
 
 struct Fp8Route {
   int q, s, e;
@@ -145,8 +145,8 @@ struct Fp8Route {
 __device__ __forceinline__ int fp8_slot_expert(const Fp8Route& r, int i, bool& bad) {
   const uint32_t q = static_cast<uint32_t>(i) / static_cast<uint32_t>(r.s);
   const int64_t t = q, s = i - static_cast<int>(q) * r.s;
+  const int64_t e = r.sel[t * r.sel_stride + s];  // both loads at once
   if (r.compute && !r.compute[t * r.compute_stride + s]) return -1;
-  const int64_t e = r.sel[t * r.sel_stride + s];
   if (e < 0 || e >= r.e) {
     bad = true;
     return -1;
@@ -154,77 +154,7 @@ __device__ __forceinline__ int fp8_slot_expert(const Fp8Route& r, int i, bool& b
   return static_cast<int>(e);
 }
 
-constexpr int kFp8PlanThreads = 1024;
-constexpr int kFp8MaxExperts = 2048;
-
-// One CTA: counts per expert, first position of each expert's slots, the slots in that order
-// (any order within an expert: a row's result does not depend on its place), and the groups
-// of at most group_rows rows of one expert: groups[i] = (expert, first position, rows, 0).
-__global__ void __launch_bounds__(kFp8PlanThreads) k_fp8_plan(Fp8Route r, int group_rows, int* sorted, int4* groups,
-                                                             int* n_groups) {
-  extern __shared__ int plan_smem[];
-  int* count = plan_smem;        // [E], then the next free position
-  int* first = plan_smem + r.e;  // [E]
-  __shared__ int s_warp[32][2];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int n = r.q * r.s;
-  for (int e = tid; e < r.e; e += kFp8PlanThreads) count[e] = 0;
-  __syncthreads();
-  bool bad = false;
-  for (int i = tid; i < n; i += kFp8PlanThreads) {
-    const int e = fp8_slot_expert(r, i, bad);
-    if (e >= 0) atomicAdd(&count[e], 1);
-  }
-  if (bad && r.err) atomicOr(r.err, static_cast<uint32_t>(kErrBadExpert));
-  __syncthreads();
-  // Exclusive prefix of (slots, groups) over the experts, two consecutive experts per thread.
-  int c[2], g[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int e = 2 * tid + j;
-    c[j] = e < r.e ? count[e] : 0;
-    g[j] = (c[j] + group_rows - 1) / group_rows;
-  }
-  int sc = c[0] + c[1], sg = g[0] + g[1];
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int pc = __shfl_up_sync(0xffffffffu, sc, o), pg = __shfl_up_sync(0xffffffffu, sg, o);
-    if (lane >= o) {
-      sc += pc;
-      sg += pg;
-    }
-  }
-  if (lane == 31) {
-    s_warp[warp][0] = sc;
-    s_warp[warp][1] = sg;
-  }
-  __syncthreads();
-  int bc = 0, bg = 0;
-  for (int w = 0; w < warp; ++w) {
-    bc += s_warp[w][0];
-    bg += s_warp[w][1];
-  }
-  int pos = bc + sc - c[0] - c[1], gi = bg + sg - g[0] - g[1];
-  if (tid == kFp8PlanThreads - 1) *n_groups = bg + sg;
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int e = 2 * tid + j;
-    if (e < r.e) {
-      first[e] = pos;
-      for (int k = 0; k < g[j]; ++k)
-        groups[gi + k] = make_int4(e, pos + k * group_rows, min(group_rows, c[j] - k * group_rows), 0);
-    }
-    pos += c[j];
-    gi += g[j];
-  }
-  __syncthreads();
-  for (int e = tid; e < r.e; e += kFp8PlanThreads) count[e] = first[e];
-  __syncthreads();
-  for (int i = tid; i < n; i += kFp8PlanThreads) {
-    const int e = fp8_slot_expert(r, i, bad);
-    if (e >= 0) sorted[atomicAdd(&count[e], 1)] = i;
-  }
-}
+constexpr int kFp8MaxExperts = 2048;  // two per thread of the plan
 
 // ---- the weight-streaming product ---------------------------------------------------------------
 //
@@ -318,7 +248,10 @@ __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+// silu(g) u with the fast exponential and division: relative error about (4 + 1.2 |g|) 2^-23 (for
+// negative g, where exp(-g) counts), far under the e4m3 rounding that follows; the exact ones took
+// 16000 cycles a tile of the many-row product. exp(-g) = inf gives 0, silu's limit.
+__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
 template <typename TX, int MODE>
 __global__ void __launch_bounds__(32 * kStreamMaxWarps) k_fp8_stream(StreamArgs a) {
@@ -464,18 +397,6 @@ __global__ void __launch_bounds__(32 * kStreamMaxWarps) k_fp8_stream(StreamArgs 
     } else {
       store_any(a.out, static_cast<int64_t>(dst) * a.out_stride + wr, v, a.out_dtype);
     }
-  }
-}
-
-// Rows of slots that are not computed, set to zero (planned batches).
-__global__ void __launch_bounds__(256) k_fp8_zero_skipped(Fp8Route r, int h, void* out, int dtype, int64_t stride_t,
-                                                         int64_t stride_s) {
-  const int n = r.q * r.s;
-  for (int i = blockIdx.x; i < n; i += gridDim.x) {
-    bool bad = false;
-    if (fp8_slot_expert(r, i, bad) >= 0) continue;
-    const int64_t o = static_cast<int64_t>(i / r.s) * stride_t + (i % r.s) * stride_s;
-    for (int j = threadIdx.x; j < h; j += blockDim.x) store_any(out, o + j, 0.f, dtype);
   }
 }
 

@@ -97,7 +97,7 @@ static int launch_tc(const CUtensorMap& xm, const CUtensorMap& wm, const F8Args&
   auto kern = k_fp8_tc<MODE>;
   const int rc = allow_smem(reinterpret_cast<const void*>(kern), kF8SmemBytes);
   if (rc) return rc;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(max_tiles, num_sms()));
+  const unsigned grid = 2 * static_cast<unsigned>(std::min<int64_t>(max_tiles, num_sms() / 2));  // pairs of CTAs
   const cudaError_t e = launch_pdl(kern, dim3(grid), dim3(kF8Threads), kF8SmemBytes, st, xm, wm, a);
   if (e != cudaSuccess) return fail(ALUT_ECUDA, "k_fp8_tc: %s", cudaGetErrorString(e));
   return ALUT_OK;
@@ -105,10 +105,16 @@ static int launch_tc(const CUtensorMap& xm, const CUtensorMap& wm, const F8Args&
 
 static int launch_rows(const F8PrepArgs& a, int x_dtype, cudaStream_t st) {
   const int64_t n = static_cast<int64_t>(a.rows) * fp8_blocks(a.k);
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((n + 15) / 16, 8 * num_sms()));
+  const unsigned grid = static_cast<unsigned>(
+      std::max<int64_t>(1, std::min<int64_t>((n + 15) / 16, std::max<int64_t>((n + 63) / 64, 4 * num_sms()))));
   auto kern = x_dtype == ALUT_BF16 ? k_fp8_rows<__nv_bfloat16> : x_dtype == ALUT_F16 ? k_fp8_rows<__half> : k_fp8_rows<float>;
-  kern<<<grid, 256, 0, st>>>(a);
-  return check_launch("k_fp8_rows");
+  if (!a.place) {
+    kern<<<grid, 256, 0, st>>>(a);
+    return check_launch("k_fp8_rows");
+  }
+  const cudaError_t e = launch_pdl(kern, dim3(grid), dim3(256), 0, st, a);
+  if (e != cudaSuccess) return fail(ALUT_ECUDA, "k_fp8_rows: %s", cudaGetErrorString(e));
+  return ALUT_OK;
 }
 
 // Which product a call takes: the weight-streaming one below these row counts.
@@ -123,7 +129,7 @@ static LinearWorkspace linear_layout(int m, int k) {
   size_t off = 0;
   if (!linear_streams(m)) {
     w.xq = off; off = align256(off + static_cast<size_t>(m) * f8_row_pitch(k));
-    w.sx = off; off = align256(off + sizeof(float) * m * f8_scale_pitch(k));
+    w.sx = off; off = align256(off + sizeof(float) * m * fp8_blocks(k));
   }
   w.total = off + 256;
   return w;
@@ -131,7 +137,7 @@ static LinearWorkspace linear_layout(int m, int k) {
 
 // Workspace of alut_experts_fp8, in order; every part starts on 256 bytes.
 struct ExpertsWorkspace {
-  size_t n_groups, groups, sorted, xq, sx, hidden, hs, total;
+  size_t n_groups, groups, sorted, place, xq, sx, hidden, hs, total;
   int64_t max_groups;
 };
 static ExpertsWorkspace experts_layout(const alut_fp8_experts_t* ex, int q, int s) {
@@ -141,14 +147,15 @@ static ExpertsWorkspace experts_layout(const alut_fp8_experts_t* ex, int q, int 
   if (experts_stream(n)) {
     w.hidden = off; off = align256(off + sizeof(float) * n * round_up(ex->i, 4));
   } else {
-    w.max_groups = ceil_div(n, kF8Rows) + std::min<int64_t>(n, ex->num_experts);
+    w.max_groups = ceil_div(n, kF8PairRows) + std::min<int64_t>(n, ex->num_experts);
     w.n_groups = off; off = align256(off + sizeof(int));
     w.groups = off;   off = align256(off + sizeof(int4) * w.max_groups);
     w.sorted = off;   off = align256(off + sizeof(int) * n);
-    w.xq = off;       off = align256(off + static_cast<size_t>(q) * f8_row_pitch(ex->h));
-    w.sx = off;       off = align256(off + sizeof(float) * q * f8_scale_pitch(ex->h));
+    w.place = off;    off = align256(off + sizeof(int) * n);
+    w.xq = off;       off = align256(off + static_cast<size_t>(n) * f8_row_pitch(ex->h));
+    w.sx = off;       off = align256(off + sizeof(float) * n * fp8_blocks(ex->h));
     w.hidden = off;   off = align256(off + static_cast<size_t>(n) * f8_row_pitch(ex->i));
-    w.hs = off;       off = align256(off + sizeof(float) * n * f8_scale_pitch(ex->i));
+    w.hs = off;       off = align256(off + sizeof(float) * n * fp8_blocks(ex->i));
   }
   w.total = off;
   return w;
@@ -223,8 +230,15 @@ int alut_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, int32_t x_dt
     if (!aligned16(workspace)) return fail(ALUT_EWORKSPACE, "linear_fp8: workspace must be 16-byte aligned");
     const LinearWorkspace ws = linear_layout(m, k);
     char* base = static_cast<char*>(workspace);
-    F8PrepArgs p{x, x_stride, m, k, rows_vec(x, x_stride, x_dtype), reinterpret_cast<uint8_t*>(base + ws.xq),
-                 reinterpret_cast<float*>(base + ws.sx)};
+    F8PrepArgs p{};
+    p.x = x;
+    p.x_stride = x_stride;
+    p.rows = m;
+    p.k = k;
+    p.x_vec = rows_vec(x, x_stride, x_dtype);
+    p.xq = reinterpret_cast<uint8_t*>(base + ws.xq);
+    p.sx = reinterpret_cast<float*>(base + ws.sx);
+    p.scale_rows = m;
     CUtensorMap xm, wm;
     rc = encode_rows(&xm, p.xq, m, k, kF8Rows);
     if (!rc) rc = encode_weight(&wm, w, k, n, 1, 1, w_stride, 0, 0);
@@ -235,13 +249,14 @@ int alut_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, int32_t x_dt
     a.n = n;
     a.k = k;
     a.sx = p.sx;
+    a.scale_rows = m;
     a.ws = w_scale;
     a.out = out;
     a.out_dtype = out_dtype;
     a.out_stride = out_stride;
     a.out_vec = rows_vec(out, out_stride, out_dtype);
     a.err = error_bits;
-    return launch_tc<kFp8Linear>(xm, wm, a, static_cast<int64_t>(ceil_div(m, kF8Rows)) * ((fp8_blocks(n) + 1) / 2), st);
+    return launch_tc<kFp8Linear>(xm, wm, a, static_cast<int64_t>(ceil_div(m, kF8PairRows)) * ((fp8_blocks(n) + 1) / 2), st);
   }
   StreamArgs a{};
   a.x = x;
@@ -290,11 +305,25 @@ int alut_experts_fp8(const alut_fp8_experts_t* ex, int32_t q, int32_t s, const v
   const int n = q * s;
   Fp8Route r{q, s, ex->num_experts, sel, sel_stride, compute, compute_stride, error_bits};
   if (!experts_stream(n)) {
-    F8PrepArgs p{x, x_stride, q, ex->h, rows_vec(x, x_stride, x_dtype), reinterpret_cast<uint8_t*>(base + ws.xq),
-                 reinterpret_cast<float*>(base + ws.sx)};
+    F8PrepArgs p{};
+    p.x = x;
+    p.x_stride = x_stride;
+    p.rows = q;
+    p.k = ex->h;
+    p.x_vec = rows_vec(x, x_stride, x_dtype);
+    p.xq = reinterpret_cast<uint8_t*>(base + ws.xq);
+    p.sx = reinterpret_cast<float*>(base + ws.sx);
+    p.scale_rows = n;
+    p.place = reinterpret_cast<int*>(base + ws.place);
+    p.s = s;
+    p.out = zero_skipped ? out : nullptr;
+    p.out_dtype = out_dtype;
+    p.out_vec = rows_vec(out, out_stride_t, out_dtype) && rows_vec(out, out_stride_s, out_dtype);
+    p.out_stride = out_stride_t;
+    p.out_stride_s = out_stride_s;
     uint8_t* hq = reinterpret_cast<uint8_t*>(base + ws.hidden);
     CUtensorMap xm, gm, hm, dm;
-    rc = encode_rows(&xm, p.xq, q, ex->h, 1);  // gathered row by row
+    rc = encode_rows(&xm, p.xq, n, ex->h, kF8Rows);
     if (!rc) rc = encode_rows(&hm, hq, n, ex->i, kF8Rows);
     if (!rc)
       rc = encode_weight(&gm, ex->gate_up, ex->h, ex->i, 2, ex->num_experts, ex->gate_up_stride[2],
@@ -306,17 +335,11 @@ int alut_experts_fp8(const alut_fp8_experts_t* ex, int32_t q, int32_t s, const v
     a.sorted = reinterpret_cast<int*>(base + ws.sorted);
     a.groups = reinterpret_cast<int4*>(base + ws.groups);
     a.n_groups = reinterpret_cast<int*>(base + ws.n_groups);
-    k_fp8_plan<<<1, kFp8PlanThreads, 2 * sizeof(int) * ex->num_experts, st>>>(
-        r, kF8Rows, reinterpret_cast<int*>(base + ws.sorted), reinterpret_cast<int4*>(base + ws.groups),
-        reinterpret_cast<int*>(base + ws.n_groups));
+    k_fp8_plan<<<kF8PlanCtas, kF8PlanThreads, 2 * sizeof(int) * ex->num_experts, st>>>(
+        r, kF8PairRows, reinterpret_cast<int*>(base + ws.sorted), reinterpret_cast<int*>(base + ws.place),
+        reinterpret_cast<int4*>(base + ws.groups), reinterpret_cast<int*>(base + ws.n_groups));
     rc = check_launch("k_fp8_plan");
     if (rc) return rc;
-    if (zero_skipped) {
-      k_fp8_zero_skipped<<<std::min(n, 16 * num_sms()), 256, 0, st>>>(r, ex->h, out, out_dtype, out_stride_t,
-                                                                     out_stride_s);
-      rc = check_launch("k_fp8_zero_skipped");
-      if (rc) return rc;
-    }
     rc = launch_rows(p, x_dtype, st);
     if (rc) return rc;
     a.s = s;
@@ -324,6 +347,7 @@ int alut_experts_fp8(const alut_fp8_experts_t* ex, int32_t q, int32_t s, const v
     a.n = ex->i;
     a.k = ex->h;
     a.sx = p.sx;
+    a.scale_rows = n;
     a.ws = ex->gate_up_scale;
     a.hq = hq;
     a.hs = reinterpret_cast<float*>(base + ws.hs);
@@ -337,7 +361,7 @@ int alut_experts_fp8(const alut_fp8_experts_t* ex, int32_t q, int32_t s, const v
     a.out_dtype = out_dtype;
     a.out_stride = out_stride_t;
     a.out_stride_s = out_stride_s;
-    a.out_vec = rows_vec(out, out_stride_t, out_dtype) && rows_vec(out, out_stride_s, out_dtype);
+    a.out_vec = p.out_vec;
     return launch_tc<kFp8Down>(hm, dm, a, ws.max_groups * ((fp8_blocks(ex->h) + 1) / 2), st);
   }
   StreamArgs a{};

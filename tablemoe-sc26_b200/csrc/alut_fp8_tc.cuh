@@ -1,25 +1,41 @@
-// The block-scaled e4m3 product for many rows: tcgen05 (kind::f8f6f4), persistent CTAs.
+// The block-scaled e4m3 product for many rows: tcgen05 (kind::f8f6f4), persistent pairs of CTAs.
 //
-// Tile: 128 rows of x (MMA M) x two 128-row weight blocks (MMA N = 256): adjacent output columns
-// (Linear, Down), or the gate and the up rows of the same 128 hidden units (GateUp).
-// The scales change with every 128 columns of K, so an accumulator holds one k-block only: the
-// MMA of a k-block (4 steps of K = 32) overwrites one of two 128 x 256 fp32 accumulators in
-// tensor memory, and the epilogue warps add it, times sx[row, block] sw[block], to fp32 registers
-// (128 a thread). Thread r of a column half owns row r, so a k-block has two factors per thread.
-// Tensor cores (512 cycles a k-block at the dense e4m3 rate) and epilogue (256 columns of TMEM
-// loads and FMAs per lane quarter) run side by side on the two accumulators.
+// Tile of a pair (cta_group::2, one MMA of M = 256, N = 256 over both SMs): 256 rows of x, 128 per
+// CTA, x two 128-row weight blocks: adjacent output columns (Linear, Down), or the gate and the up
+// rows of the same 128 hidden units (GateUp). Each CTA loads its own rows of x and one of the two
+// weight blocks: 32 KB per 128 columns of K and CTA. With one CTA per tile it is 48 KB, and the
+// copies out of L2 and the operands' way through shared memory (48 KB in, 48 KB out, 128 bytes a
+// cycle) set the rate: 1040 cycles a k-block measured against 512 of the tensor cores.
+// The scales change with every 128 columns of K, so an accumulator holds one k-block only: the MMAs
+// of a k-block (4 steps of K = 32) overwrite it, and the epilogue warps add it, times sx[row, block]
+// sw[block], to fp32 registers (128 a thread; a thread owns a row: two factors per k-block). Tensor
+// memory holds four accumulators of 128 columns, half a k-block's: the low or high 64 rows of both
+// weight blocks (an MMA of N = 128 takes 64 rows from each CTA). What bounds it, measured: the MMAs
+// alone 515 cycles a k-block, with the copies 522; but a k-block's MMA is done 950 cycles after its
+// issue, and reading it back (128 KB per SM through the TMEM port) takes 540. With two accumulators
+// of a whole k-block that chain ran at 1000 cycles a k-block.
 //
-//   warps 0-7  epilogue: TMEM lane quarter warp % 4, columns 64 (warp / 4) .. + 64 of each block
-//   warp 8     copies: both operands by TMA with the 128-byte swizzle; GateUp gathers x's rows
-//              by token (one tile::gather4 of 4 rows per lane and k-block)
-//   warp 9     MMA issuer (10, 11 idle: registers are handed over by warpgroups)
-//   barriers:  full/empty per stage, full/empty per accumulator
+//   warps 0-7  epilogue: TMEM lane quarter warp % 4, columns 32 (warp / 4) .. + 32 of each 64
+//   warp 8     TMA copies (128-byte swizzle), signalled to the leader CTA's barrier
+//   warp 9     MMA issuer (of the pair's leader, rank 0)
+//   warp 10    the factors sx sw of a k-block's 128 rows and two blocks, into a ring in shared
+//              memory (read by the epilogue itself, their latency cost 460 cycles a k-block)
+//   warp 11    waits for the accumulators and lets the epilogue go by a named barrier: of warps
+//              that waited on the mbarrier themselves the last woke 600 cycles after the first
+//   barriers:  full/empty per stage, full/empty per accumulator, full/empty per ring slot; the
+//              stages' full and the accumulators' empty count in the leader, the commits arrive in
+//              both CTAs
 // GateUp ends with h = silu(gate) * up, its 8-bit form (the 128 hidden units of the tile are one
 // block of the next product; the two column halves exchange their maxima) written for Down.
-// Every wait is bounded in time (error bit, stop, bounded drain, TMEM freed).
+// x's rows lie in the order of the plan (k_fp8_rows writes a token's 8-bit row once per computed
+// slot), so all three products load plain tiles: gathering the rows here was slower (tile::gather4
+// moves a 128-byte row every 13 ns, 1.7 us a k-block; 16-byte cp.async by two warps 1.5 us).
+// Every wait is bounded in time (error bit, stop, time for what is in flight, TMEM freed).
 #pragma once
 
 #include <cuda.h>
+
+#include <cooperative_groups.h>
 
 #include "alut_common.cuh"
 #include "alut_fp8.cuh"
@@ -27,345 +43,546 @@
 
 namespace alut {
 
-constexpr int kF8Rows = 128;
-constexpr int kF8Stages = 4;
+constexpr int kF8Rows = 128;                // rows of x per CTA
+constexpr int kF8PairRows = 2 * kF8Rows;    // per pair of CTAs
+constexpr int kF8Stages = 6;
 constexpr uint32_t kF8TileBytes = kF8Rows * kFp8Block;  // one 128 x 128 operand tile
-constexpr uint32_t kF8StageBytes = 3 * kF8TileBytes;    // x, two weight blocks
+constexpr uint32_t kF8StageBytes = 2 * kF8TileBytes;    // x's rows, a weight block
 constexpr int kF8EpiWarps = 8;
-// Three warpgroups of 128 threads, launched with 168 registers a thread; the epilogue's two need
-// more (128 sums, 64 loaded values), the third fewer: 2 x 232 + 40 = 3 x 168.
+// Three warpgroups, launched with 168 registers a thread; the epilogue's two need more (128 sums, 64
+// loaded values), the third fewer: 2 x 232 + 40 = 3 x 168.
 constexpr int kF8Threads = 32 * (kF8EpiWarps + 4);
 constexpr int kF8EpiRegs = 232, kF8RoleRegs = 40;
-constexpr int kF8CopyWarp = kF8EpiWarps, kF8MmaWarp = kF8EpiWarps + 1;
+constexpr int kF8CopyWarp = kF8EpiWarps, kF8MmaWarp = kF8EpiWarps + 1, kF8ScaleWarp = kF8EpiWarps + 2, kF8WaitWarp = kF8EpiWarps + 3;
+constexpr int kF8Group = 4, kF8Ring = 2;     // factors of 4 k-blocks per ring slot
+constexpr uint32_t kF8StoreBytes = 32 * 64;  // a warp's output rows on their way out
 constexpr uint32_t kF8TmemCols = 512;
-constexpr size_t kF8SmemBytes = 1024 + 1024 + static_cast<size_t>(kF8Stages) * kF8StageBytes;
+constexpr int kF8Acc = 4, kF8AccCols = 128;  // accumulators
+constexpr size_t kF8SmemBytes = 1024 + 1024 + static_cast<size_t>(kF8Stages) * kF8StageBytes +
+                                kF8EpiWarps * kF8StoreBytes + kF8Ring * kF8Group * kF8Rows * sizeof(float2);
 
-// Scales of x's rows (and of the hidden rows) are kept [row][blocks rounded up to 4].
-__host__ __device__ inline int f8_scale_pitch(int k) { return (fp8_blocks(k) + 3) & ~3; }
+// Scales of x's rows (and of the hidden rows) are kept [block][row]: a k-block's are adjacent.
 __host__ __device__ inline int64_t f8_row_pitch(int k) { return static_cast<int64_t>(fp8_blocks(k)) * kFp8Block; }
 
 struct F8Args {
   int m, n, k;              // rows (Linear), weight rows per half, reduction length
-  const float* sx;          // x's scales [rows][f8_scale_pitch(k)]
+  const float* sx;          // x's scales [blocks k][scale_rows]
+  int64_t scale_rows;       // rows (positions) in all
   const float* ws;          // weight scales, contiguous [E][halves][blocks n][blocks k]
   const int4* groups;       // GateUp, Down: (expert, first position, rows, 0)
   const int* n_groups;
   const int* sorted;        // position -> slot
   int s;                    // slots per token
   uint8_t* hq;              // GateUp: [positions][f8_row_pitch(n)]
-  float* hs;                // GateUp: [positions][f8_scale_pitch(n)]
+  float* hs;                // GateUp: [blocks n][scale_rows]
   void* out;                // Linear [m, n], Down [q, s, n]
   int out_dtype, out_vec;   // out_vec: 16-byte stores are aligned
   int64_t out_stride, out_stride_s;
   uint32_t* err;
 };
 
-__device__ __forceinline__ void f8_load_tile(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-  pt_tma_load_2d(dst, map, x, y, bar);
+// The same shared variable of the pair's CTA `rank`, as a shared::cluster address.
+__device__ __forceinline__ uint32_t f8_of_rank(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
+  return r;
+}
+// No memory is handed over with this arrival (the accumulator was read, tcgen05 fences order that);
+// with .release.cluster each one waited for the warp's memory traffic: 2 x the whole product's time.
+__device__ __forceinline__ void f8_arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Waits on a barrier of this CTA (by its shared address). A wait that runs out (1 s), or that another
+// role has given up, returns as if it were over: the flag and the error bit say so, each role stops
+// at its next tile, and what it does until then stays in bounds. The timer is read only every 256
+// tries: a read of %globaltimer takes most of a microsecond.
+__device__ __forceinline__ bool f8_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void f8_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t* err) {
+  uint64_t t0 = 0;
+  for (uint32_t n = 1; !f8_try(bar, parity); ++n) {
+    if (n & 255) continue;
+    if (*abort_flag) return;
+    const uint64_t now = global_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > kWaitNs) {
+      *abort_flag = 1;
+      if (err) atomicOr(err, static_cast<uint32_t>(kErrMmaTimeout));
+      return;
+    }
+  }
+}
+// One lane of a converged warp, chosen so that the compiler knows it is one: the operands of the
+// MMAs and copies then stay in uniform registers (behind lane == 0 the issue of a k-block's four
+// MMAs and two commits took 600 cycles).
+__device__ __forceinline__ bool f8_elect() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ void f8_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// TMA copies into this CTA's shared memory whose bytes count on a barrier of either CTA of the pair.
+__device__ __forceinline__ void f8_load_rows(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3}], [%4];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
 }
 __device__ __forceinline__ void f8_load_weight(void* dst, const CUtensorMap* map, int x, int y, int half, int e,
-                                               uint64_t* bar) {
+                                               uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-      "[%6];" ::"r"(smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(half), "r"(e), "r"(smem_addr(bar))
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3, %4, %5}], [%6];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(half), "r"(e), "r"(bar)
       : "memory");
 }
-// Four rows (128 bytes each) of a map whose box is one row high.
-__device__ __forceinline__ void f8_gather4(void* dst, const CUtensorMap* map, int x, int4 rows, uint64_t* bar) {
+__device__ __forceinline__ void f8_commit(uint64_t* bar) {  // arrives on `bar` of both CTAs
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
-      "%4, %5, %6}], [%7];" ::"r"(smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w),
-      "r"(smem_addr(bar))
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_addr(bar)),
+      "h"(static_cast<uint16_t>(3))
       : "memory");
 }
-// kind::f8f6f4 instruction descriptor: fp32 D, e4m3 A and B, K-major, M = 128, N = 256.
+// kind::f8f6f4 instruction descriptor: fp32 D, e4m3 A and B, K-major, M = 256, N = 128.
 __host__ __device__ __forceinline__ uint32_t f8_idesc() {
-  return (1u << 4) | (static_cast<uint32_t>(256 >> 3) << 17) | (static_cast<uint32_t>(kF8Rows >> 4) << 24);
+  return (1u << 4) | (static_cast<uint32_t>(kF8AccCols >> 3) << 17) | (static_cast<uint32_t>(kF8PairRows >> 4) << 24);
 }
 __device__ __forceinline__ void f8_mma(uint32_t tmem, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(
           tmem),
       "l"(da), "l"(db), "r"(idesc), "r"(acc)
       : "memory");
 }
 
-// 64 fp32 values as consecutive outputs of a row, columns c .. c + 63 of n.
-__device__ __forceinline__ void f8_store64(void* out, int64_t o, const float (&v)[64], int c, int n, int dtype, bool vec) {
-  if (vec && c + 64 <= n && dtype != ALUT_F32) {
+// 32 columns of this warp's 32 TMEM lanes, not waited for: the registers hold them after f8_ld_wait.
+__device__ __forceinline__ void f8_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%"
+      "19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+// Waits for this warp's loads; taking the registers in and out keeps every use behind it.
+__device__ __forceinline__ void f8_ld_wait(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29])
+               :
+               : "memory");
+  asm volatile("" : "+r"(r[30]), "+r"(r[31]));
+}
+// sum[j] += f * (the loaded column j). (The packed fma.rn.f32x2 is no help: it runs on one of the
+// two fp32 pipes.)
+__device__ __forceinline__ void f8_accumulate(float (&sum)[32], const uint32_t (&r)[32], float f) {
 #pragma unroll
-    for (int j = 0; j < 64; j += 8) {
-      const float (&w)[8] = reinterpret_cast<const float (&)[8]>(v[j]);
-      if (dtype == ALUT_BF16) store8<__nv_bfloat16>(static_cast<__nv_bfloat16*>(out) + o + j, w);
-      else store8<__half>(static_cast<__half*>(out) + o + j, w);
-    }
-    return;
+  for (int j = 0; j < 32; ++j) sum[j] = fmaf(__uint_as_float(r[j]), f, sum[j]);
+}
+
+// 16-byte unit c of row r in a warp's 32 x 64-byte buffer: rows and columns without bank conflicts.
+__device__ __forceinline__ uint32_t f8_unit(int r, int c) {
+  return static_cast<uint32_t>(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+}
+
+// A warp's 32 rows x C columns (lane r has row r's values v and its output offset o, negative for
+// no row) out through shared memory, so that a store instruction writes 64 adjacent bytes of 8 rows
+// (a row per thread writes 32 half sectors at a time).
+template <typename TO, int C>
+__device__ __forceinline__ void f8_store(TO* out, int64_t o, const float* v, int c0, int n, bool vec, unsigned char* buf) {
+  static_assert(C * sizeof(TO) == 64, "a buffer row");
+  const int lane = threadIdx.x & 31;
+  constexpr int kPer = 16 / sizeof(TO);
+  __syncwarp();
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    __align__(16) TO t[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) t[j] = from_f32<TO>(v[c * kPer + j]);
+    *reinterpret_cast<uint4*>(buf + f8_unit(lane, c)) = *reinterpret_cast<const uint4*>(t);
   }
+  __syncwarp();
+  if (vec && c0 + C <= n) {
 #pragma unroll
-  for (int j = 0; j < 64; ++j)
-    if (c + j < n) store_any(out, o + j, v[j], dtype);
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + (lane >> 2);
+      const int64_t ro = __shfl_sync(0xffffffffu, o, r);
+      const uint4 u = *reinterpret_cast<const uint4*>(buf + f8_unit(r, lane & 3));
+      if (ro >= 0) *reinterpret_cast<uint4*>(out + ro + c0 + (lane & 3) * kPer) = u;
+    }
+  } else {  // a ragged edge, or rows that do not start on 16 bytes: element by element along the row
+    for (int r = 0; r < 32; ++r) {
+      const int64_t ro = __shfl_sync(0xffffffffu, o, r);
+      if (ro >= 0 && lane < C && c0 + lane < n)
+        out[ro + c0 + lane] = *reinterpret_cast<const TO*>(buf + f8_unit(r, lane / kPer) + (lane % kPer) * sizeof(TO));
+    }
+  }
+}
+__device__ __forceinline__ void f8_store32(void* out, int64_t o, const float (&v)[32], int c, int n, int dtype, bool vec,
+                                           unsigned char* buf) {
+  if (dtype == ALUT_BF16) {
+    f8_store<__nv_bfloat16, 32>(static_cast<__nv_bfloat16*>(out), o, v, c, n, vec, buf);
+  } else if (dtype == ALUT_F16) {
+    f8_store<__half, 32>(static_cast<__half*>(out), o, v, c, n, vec, buf);
+  } else {
+    f8_store<float, 16>(static_cast<float*>(out), o, v, c, n, vec, buf);
+    f8_store<float, 16>(static_cast<float*>(out), o, v + 16, c + 16, n, vec, buf);
+  }
 }
 
 template <int MODE>
-__global__ void __launch_bounds__(kF8Threads, 1)
+__global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
     k_fp8_tc(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, F8Args a) {
   extern __shared__ unsigned char f8_raw[];
   unsigned char* f8_smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(f8_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(f8_smem);  // [kF8Stages]
+  uint64_t* full = reinterpret_cast<uint64_t*>(f8_smem);  // [kF8Stages] (the leader's counts for the pair)
   uint64_t* empty = full + kF8Stages;                     // [kF8Stages]
-  uint64_t* t_full = empty + kF8Stages;                   // [2]
-  uint64_t* t_empty = t_full + 2;                         // [2]
-  uint64_t* maxima = t_empty + 2;                         // [1] both column halves' maxima are there
-  uint64_t* drain = maxima + 1;                           // [1]
-  unsigned char* stages = f8_smem + 1024;                 // [kF8Stages][x | block 0 | block 1]
+  uint64_t* t_full = empty + kF8Stages;                   // [kF8Acc]
+  uint64_t* t_empty = t_full + kF8Acc;                    // [kF8Acc] (the leader's counts for the pair)
+  uint64_t* maxima = t_empty + kF8Acc;                    // [1] both column parts' maxima are there
+  uint64_t* f_full = maxima + 1;                          // [kF8Ring]
+  uint64_t* f_empty = f_full + kF8Ring;                   // [kF8Ring]
+  unsigned char* stages = f8_smem + 1024;                 // [kF8Stages][x rows | weight block]
+  unsigned char* out_buf = stages + kF8Stages * static_cast<size_t>(kF8StageBytes);  // [kF8EpiWarps][kF8StoreBytes]
+  float2* ring = reinterpret_cast<float2*>(out_buf + kF8EpiWarps * kF8StoreBytes);    // [kF8Ring][kF8Group][kF8Rows]
   __shared__ float s_max[2][2][kF8Rows];                  // [tile parity][column half][row]
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort, s_issued;
+  __shared__ int s_abort;
   volatile int* abort_flag = &s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = blockIdx.x & 1;  // in the pair
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
   const int kblocks = fp8_blocks(a.k), nblocks = fp8_blocks(a.n);
   pdl_launch_dependents();
   if (warp == kF8MmaWarp) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)),
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)),
                  "r"(kF8TmemCols)
                  : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   if (tid == 0) {
     for (int i = 0; i < kF8Stages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kF8Acc; ++i) {
       mbar_init(&t_full[i], 1);
-      mbar_init(&t_empty[i], kF8EpiWarps);
+      mbar_init(&t_empty[i], 2 * kF8EpiWarps);
     }
     mbar_init(maxima, kF8EpiWarps);
-    mbar_init(drain, 1);
+    for (int i = 0; i < kF8Ring; ++i) {
+      mbar_init(&f_full[i], 1);
+      mbar_init(&f_empty[i], kF8EpiWarps);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_abort = 0;
-    s_issued = 0;
   }
   tc_fence_before();
   __syncthreads();
+  f8_cluster_sync();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
   pdl_wait();  // the 8-bit rows, the plan and the scales come from the kernel before
   const int nt = MODE == kFp8GateUp ? nblocks : (nblocks + 1) / 2;  // tiles along the weight rows
-  const int mt = MODE == kFp8Linear ? (a.m + kF8Rows - 1) / kF8Rows : __ldcg(a.n_groups);
+  const int mt = MODE == kFp8Linear ? (a.m + kF8PairRows - 1) / kF8PairRows : __ldcg(a.n_groups);
   const int64_t ntiles = static_cast<int64_t>(mt) * nt;
+  // A pair tile: expert, first row (position) and number of rows.
+  auto tile_rows = [&](int mi) {
+    if constexpr (MODE == kFp8Linear) return make_int4(0, mi * kF8PairRows, min(kF8PairRows, a.m - mi * kF8PairRows), 0);
+    else return __ldcg(a.groups + mi);
+  };
 
+  auto wait = [&](uint64_t* bars, int i, uint32_t parity) {  // a fresh barrier counts as past parity 1
+    f8_wait(smem_addr(bars) + 8 * i, parity, abort_flag, a.err);
+  };
+  auto stopped = [&]() { return __any_sync(0xffffffffu, *abort_flag); };
+
+  // Every role is a whole warp that walks the same tiles; one elected lane issues.
   if (warp >= kF8EpiWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kF8RoleRegs));
     if (warp == kF8CopyWarp) {
-      // ---- copies ------------------------------------------------------------------------------
-      int it = 0, st = 0, wrapped = 0;
-      bool ok = true;
-      for (int64_t tile = blockIdx.x; tile < ntiles && ok; tile += gridDim.x) {
+      // ---- TMA copies --------------------------------------------------------------------------
+      int st = 0, past = 1;
+      for (int64_t tile = pair; tile < ntiles && !stopped(); tile += npairs) {
         const int mi = static_cast<int>(tile / nt), ni = static_cast<int>(tile % nt);
-        int e = 0, row0 = mi * kF8Rows;
-        int4 rows = make_int4(0, 0, 0, 0);
-        if constexpr (MODE != kFp8Linear) {
-          const int4 g = __ldcg(a.groups + mi);
-          e = g.x;
-          row0 = g.y;
-          if constexpr (MODE == kFp8GateUp) {  // this lane's four rows; rows past the group repeat its first
-            int* r = reinterpret_cast<int*>(&rows);
-  #pragma unroll
-            for (int j = 0; j < 4; ++j) r[j] = __ldcg(a.sorted + g.y + (4 * lane + j < g.z ? 4 * lane + j : 0)) / a.s;
+        const int4 g = tile_rows(mi);
+        const bool second = g.z > kF8Rows;  // the second CTA has rows
+        const uint32_t bytes = kF8TileBytes * (second ? 4 : 3);
+        const int wrow = MODE == kFp8GateUp ? ni * kFp8Block : (2 * ni + static_cast<int>(rank)) * kFp8Block;
+        const int half = MODE == kFp8GateUp ? static_cast<int>(rank) : 0;
+        const int xrow = g.y + static_cast<int>(rank) * kF8Rows;
+        for (int kb = 0; kb < kblocks; ++kb, (++st == kF8Stages ? (st = 0, past ^= 1) : 0)) {
+          wait(empty, st, past);
+          if (f8_elect()) {
+            unsigned char* sx = stages + static_cast<size_t>(st) * kF8StageBytes;
+            const uint32_t bar = f8_of_rank(&full[st], 0);
+            if (rank == 0) mbar_expect_tx(&full[st], bytes);
+            f8_load_weight(sx + kF8TileBytes, &w_map, kb * kFp8Block, wrow, half, g.x, bar);
+            if (rank == 0 || second) f8_load_rows(sx, &x_map, kb * kFp8Block, xrow, bar);
           }
-        }
-        for (int kb = 0; kb < kblocks; ++kb, ++it, (++st == kF8Stages ? (st = 0, wrapped ^= 1) : 0)) {
-          if (lane == 0 && it >= kF8Stages) ok = tc_wait(&empty[st], wrapped ^ 1, abort_flag);
-          ok = __shfl_sync(0xffffffffu, ok, 0);
-          if (!ok) break;
-          unsigned char* sx = stages + static_cast<size_t>(st) * kF8StageBytes;
-          if (lane == 0) {
-            mbar_expect_tx(&full[st], kF8StageBytes);
-            if constexpr (MODE == kFp8GateUp) {
-              f8_load_weight(sx + kF8TileBytes, &w_map, kb * kFp8Block, ni * kFp8Block, 0, e, &full[st]);
-              f8_load_weight(sx + 2 * kF8TileBytes, &w_map, kb * kFp8Block, ni * kFp8Block, 1, e, &full[st]);
-            } else {
-              f8_load_tile(sx, &x_map, kb * kFp8Block, row0, &full[st]);
-              f8_load_weight(sx + kF8TileBytes, &w_map, kb * kFp8Block, 2 * ni * kFp8Block, 0, e, &full[st]);
-              f8_load_weight(sx + 2 * kF8TileBytes, &w_map, kb * kFp8Block, (2 * ni + 1) * kFp8Block, 0, e, &full[st]);
-            }
-          }
-          if constexpr (MODE == kFp8GateUp) {
-            __syncwarp();
-            f8_gather4(sx + lane * 4 * kFp8Block, &x_map, kb * kFp8Block, rows, &full[st]);
-          }
-        }
-      }
-      if (lane == 0) {
-        s_issued = it;
-        if (!ok && !*abort_flag) {
-          *abort_flag = 1;
-          if (a.err) atomicOr(a.err, static_cast<uint32_t>(kErrMmaTimeout));
+          __syncwarp();
         }
       }
     } else if (warp == kF8MmaWarp) {
       // ---- MMA issuer ----------------------------------------------------------------------------
-      if (lane == 0) {
-        int it = 0, st = 0, sph = 0;
-        bool ok = true;
+      if (rank == 0) {
+        int st = 0, ph = 0, buf = 0, past = 1;
         const uint32_t idesc = f8_idesc();
-        for (int64_t tile = blockIdx.x; tile < ntiles && ok; tile += gridDim.x) {
-          for (int kb = 0; kb < kblocks; ++kb, ++it, (++st == kF8Stages ? (st = 0, sph ^= 1) : 0)) {
-            const int buf = it & 1;
-            if ((it >= 2 && !tc_wait(&t_empty[buf], ((it >> 1) - 1) & 1, abort_flag)) ||
-                !tc_wait(&full[st], sph, abort_flag)) {
-              ok = false;
-              break;
+        const uint64_t desc0 = pt_desc_sw128(smem_addr(stages));  // + address / 16 within the first 14 bits
+        for (int64_t tile = pair; tile < ntiles && !stopped(); tile += npairs) {
+          for (int kb = 0; kb < kblocks; ++kb) {
+            wait(full, st, ph);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {  // accumulator 2 buf + h, used once per two k-blocks
+              const int acc = 2 * buf + h;
+              wait(t_empty, acc, past);
+              tc_fence_after();
+              if (f8_elect()) {
+                const uint64_t dx = desc0 + static_cast<uint32_t>(st) * (kF8StageBytes >> 4);
+                const uint64_t dw = dx + ((kF8TileBytes + h * kF8TileBytes / 2) >> 4);
+#pragma unroll
+                for (int k32 = 0; k32 < kFp8Block / 32; ++k32)
+                  f8_mma(tmem + acc * kF8AccCols, dx + 2 * k32, dw + 2 * k32, idesc, k32 ? 1u : 0u);
+                f8_commit(&t_full[acc]);
+                if (h) f8_commit(&empty[st]);
+              }
+              __syncwarp();
             }
-            tc_fence_after();
-            const uint32_t sx = smem_addr(stages + static_cast<size_t>(st) * kF8StageBytes);
-  #pragma unroll
-            for (int k32 = 0; k32 < kFp8Block / 32; ++k32)
-              f8_mma(tmem + buf * 256, pt_desc_sw128(sx + k32 * 32), pt_desc_sw128(sx + kF8TileBytes + k32 * 32), idesc,
-                     k32 ? 1u : 0u);
-            tc_commit(&empty[st]);
-            tc_commit(&t_full[buf]);
+            if (++st == kF8Stages) {
+              st = 0;
+              ph ^= 1;
+            }
+            past ^= buf;
+            buf ^= 1;
           }
         }
-        if (!ok && !*abort_flag) {
-          *abort_flag = 1;
-          if (a.err) atomicOr(a.err, static_cast<uint32_t>(kErrMmaTimeout));
+      }
+    } else if (warp == kF8ScaleWarp) {
+      // ---- factors -----------------------------------------------------------------------------
+      int sl = 0, past = 1;
+      for (int64_t tile = pair; tile < ntiles && !stopped(); tile += npairs) {
+        const int mi = static_cast<int>(tile / nt), ni = static_cast<int>(tile % nt);
+        const int4 g = tile_rows(mi);
+        const int rows = min(kF8Rows, g.z - static_cast<int>(rank) * kF8Rows);  // may be <= 0
+        const float* sx = a.sx + g.y + rank * kF8Rows + lane;
+        const int nb0 = MODE == kFp8GateUp ? ni : 2 * ni;
+        const float* sw0 = a.ws + (static_cast<int64_t>(g.x) * (MODE == kFp8GateUp ? 2 : 1) * nblocks + nb0) * kblocks;
+        // the second block: the up rows' scales, or the next block of columns (none past the last)
+        const float* sw1 = MODE == kFp8GateUp ? sw0 + static_cast<int64_t>(nblocks) * kblocks
+                                              : (nb0 + 1 < nblocks ? sw0 + kblocks : sw0);
+        for (int kb = 0; kb < kblocks; ++kb) {
+          float s[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[j] = lane + 32 * j < rows ? __ldcg(sx + 32 * j) : 0.f;
+          const float w0 = __ldg(sw0 + kb), w1 = __ldg(sw1 + kb);
+          sx += a.scale_rows;
+          const int in = kb & (kF8Group - 1);
+          if (in == 0) wait(f_empty, sl, past);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            ring[(sl * kF8Group + in) * kF8Rows + lane + 32 * j] = make_float2(s[j] * w0, s[j] * w1);
+          if (in == kF8Group - 1 || kb == kblocks - 1) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&f_full[sl]);
+            if (++sl == kF8Ring) {
+              sl = 0;
+              past ^= 1;
+            }
+          }
         }
       }
+    } else {
+      // ---- accumulators (and their factors) done: let the epilogue go ------------------------------
+      // It and the epilogue run through every tile even after an abort, without waiting then: a
+      // named barrier's counts have to match.
+      int sl = 0, sph = 0, buf = 0, ph = 0;
+      for (int64_t tile = pair; tile < ntiles; tile += npairs)
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if ((kb & (kF8Group - 1)) == 0) {
+            if (!*abort_flag) wait(f_full, sl, sph);
+            if (++sl == kF8Ring) {
+              sl = 0;
+              sph ^= 1;
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (!*abort_flag) wait(t_full, 2 * buf + h, ph);
+            __syncwarp();
+            asm volatile("bar.arrive %0, %1;" ::"r"(1 + 2 * buf + h), "n"(32 * (kF8EpiWarps + 1)) : "memory");
+          }
+          ph ^= buf;
+          buf ^= 1;
+        }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kF8EpiRegs));
     // ---- epilogue ------------------------------------------------------------------------------
-    const int half = warp >> 2;
-    const int row = (warp & 3) * 32 + lane;
-    const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + half * 64;
-    const int pitch = f8_scale_pitch(a.k);
-    int it = 0, par = 0;
-    bool ok = true;
-    auto stop_if = [&](bool bad) {  // whole warps: a wait ran out
-      bad = __any_sync(0xffffffffu, bad);
-      if (bad && lane == 0 && !*abort_flag) {
-        *abort_flag = 1;
-        if (a.err) atomicOr(a.err, static_cast<uint32_t>(kErrMmaTimeout));
-      }
-      return bad;
+    const int part = warp >> 2;
+    const int warp_row = (warp & 3) * 32, row = warp_row + lane;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp_row) << 16) + part * 32;
+    const uint32_t released = f8_of_rank(&t_empty[0], 0);
+    unsigned char* buf_out = out_buf + warp * kF8StoreBytes;
+    int buf = 0, sl = 0, par = 0;
+    auto ready = [&](int ac) {
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + ac), "n"(32 * (kF8EpiWarps + 1)) : "memory");
+      tc_fence_after();
     };
-    for (int64_t tile = blockIdx.x; tile < ntiles && ok; tile += gridDim.x, par ^= 1) {
+    auto release = [&](int ac) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) f8_arrive_remote(released + 8 * ac);
+    };
+    auto group_read = [&](int kb) {  // this warp has the factors of k-block kb: its group's last?
+      if ((kb & (kF8Group - 1)) == kF8Group - 1 || kb == kblocks - 1) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&f_empty[sl]);
+        if (++sl == kF8Ring) sl = 0;
+      }
+    };
+    for (int64_t tile = pair; tile < ntiles; tile += npairs, par ^= 1) {
       const int mi = static_cast<int>(tile / nt), ni = static_cast<int>(tile % nt);
-      int e = 0, rows, pos0 = mi * kF8Rows;
-      if constexpr (MODE == kFp8Linear) {
-        rows = min(kF8Rows, a.m - pos0);
-      } else {
-        const int4 g = __ldcg(a.groups + mi);
-        e = g.x;
-        pos0 = g.y;
-        rows = g.z;
-      }
-      const bool live = row < rows;
-      int src = pos0 + (live ? row : 0);
-      int slot = 0;
-      if constexpr (MODE != kFp8Linear) slot = __ldcg(a.sorted + src);
-      if constexpr (MODE == kFp8GateUp) src = slot / a.s;
-      const float4* sxp = reinterpret_cast<const float4*>(a.sx + static_cast<int64_t>(src) * pitch);
-      const int nb0 = MODE == kFp8GateUp ? ni : 2 * ni;
-      const float* sw0 = a.ws + ((static_cast<int64_t>(e) * (MODE == kFp8GateUp ? 2 : 1)) * nblocks + nb0) * kblocks;
-      // the second block: the up rows' scales, or the next block of columns (none past the last)
-      const float* sw1 = MODE == kFp8GateUp ? sw0 + static_cast<int64_t>(nblocks) * kblocks
-                                            : (nb0 + 1 < nblocks ? sw0 + kblocks : sw0);
-      float acc0[64], acc1[64];
+      const int4 g = tile_rows(mi);
+      const int pos0 = g.y + static_cast<int>(rank) * kF8Rows;
+      const int rows = g.z - static_cast<int>(rank) * kF8Rows;  // of this CTA; may be <= 0
+      const bool live = row < rows, warp_live = warp_row < rows;
+      float acc[2][2][32];  // [block][half][column]: column 64 half + 32 part + j of the block
 #pragma unroll
-      for (int j = 0; j < 64; ++j) acc0[j] = acc1[j] = 0.f;
-      float4 s4 = __ldcg(sxp);
-      float w0 = __ldg(sw0), w1 = __ldg(sw1);
-      for (int kb = 0; kb < kblocks; ++kb, ++it) {
-        const int buf = it & 1;
-        const float s = (kb & 3) == 0 ? s4.x : (kb & 3) == 1 ? s4.y : (kb & 3) == 2 ? s4.z : s4.w;
-        const float f0 = s * w0, f1 = s * w1;
-        if (kb + 1 < kblocks) {  // the next block's factors, a k-block ahead
-          if (((kb + 1) & 3) == 0) s4 = __ldcg(sxp + ((kb + 1) >> 2));
-          w0 = __ldg(sw0 + kb + 1);
-          w1 = __ldg(sw1 + kb + 1);
-        }
-        if (stop_if(!tc_wait(&t_full[buf], (it >> 1) & 1, abort_flag))) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float v[32];
-          tc_ld32(lane_base + buf * 256 + (c >> 1) * 128 + (c & 1) * 32, v);
-          if (c == 3) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&t_empty[buf]);
+      for (int j = 0; j < 32; ++j) acc[0][0][j] = acc[0][1][j] = acc[1][0][j] = acc[1][1][j] = 0.f;
+      if (warp_live) {
+        // A load is under way while the registers of the one before are added up: the next
+        // accumulator's first 32 columns behind this one's, the last 32 behind those.
+        uint32_t v0[32], v1[32];
+        const float2* fr = ring + row;
+        float2 f, fn = make_float2(0.f, 0.f);
+        ready(2 * buf);
+        f = fr[sl * kF8Group * kF8Rows];
+        group_read(0);
+        f8_ld32(lane_base + 2 * buf * kF8AccCols, v0);
+        f8_ld32(lane_base + 2 * buf * kF8AccCols + 64, v1);
+        for (int kb = 0; kb < kblocks; ++kb) {
+          const uint32_t d = lane_base + 2 * buf * kF8AccCols, dn = lane_base + 2 * (buf ^ 1) * kF8AccCols;
+          f8_ld_wait(v0);
+          f8_ld_wait(v1);
+          release(2 * buf);
+          f8_accumulate(acc[0][0], v0, f.x);
+          ready(2 * buf + 1);
+          f8_ld32(d + kF8AccCols, v0);
+          f8_accumulate(acc[1][0], v1, f.y);
+          f8_ld32(d + kF8AccCols + 64, v1);
+          f8_ld_wait(v0);
+          f8_ld_wait(v1);
+          release(2 * buf + 1);
+          f8_accumulate(acc[0][1], v0, f.x);
+          const bool more = kb + 1 < kblocks;
+          if (more) {
+            ready(2 * (buf ^ 1));
+            fn = fr[(sl * kF8Group + ((kb + 1) & (kF8Group - 1))) * kF8Rows];
+            group_read(kb + 1);
+            f8_ld32(dn, v0);
           }
+          f8_accumulate(acc[1][1], v1, f.y);
+          if (more) f8_ld32(dn + 64, v1);
+          f = fn;
+          buf ^= 1;
+        }
+      } else {  // no row here: nothing to read
+        for (int kb = 0; kb < kblocks; ++kb, buf ^= 1) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            if (c < 2) acc0[c * 32 + j] = fmaf(v[j], f0, acc0[c * 32 + j]);
-            else acc1[(c - 2) * 32 + j] = fmaf(v[j], f1, acc1[(c - 2) * 32 + j]);
+          for (int h = 0; h < 2; ++h) {
+            ready(2 * buf + h);
+            release(2 * buf + h);
           }
+          group_read(kb);
         }
       }
-      if (!ok) break;
       if constexpr (MODE == kFp8GateUp) {
         uint32_t m = 0;
 #pragma unroll
-        for (int j = 0; j < 64; ++j) {  // columns past I have zero weights: h = 0
-          acc0[j] = silu_mul(acc0[j], acc1[j]);
-          m = max(m, abs_bits(acc0[j]));
-        }
-        s_max[par][half][row] = __uint_as_float(m);
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {  // columns past I have zero weights: h = 0
+            acc[0][h][j] = silu_mul(acc[0][h][j], acc[1][h][j]);
+            m = max(m, abs_bits(acc[0][h][j]));
+          }
+        s_max[par][part][row] = __uint_as_float(m);
         __syncwarp();
         if (lane == 0) mbar_arrive(maxima);
-        if (stop_if(!tc_wait(maxima, par, abort_flag))) break;
-        m = max(m, __float_as_uint(s_max[par][half ^ 1][row]));
+        if (!*abort_flag) wait(maxima, 0, par);
+        m = max(m, __float_as_uint(s_max[par][part ^ 1][row]));
         const float am = fp8_amax(m);
         const float f = kE4m3Max / am;
-        if (live) {
-          const int64_t pos = pos0 + row;
-          uint4* dst = reinterpret_cast<uint4*>(a.hq + pos * f8_row_pitch(a.n) + ni * kFp8Block + half * 64);
+        __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+        for (int h = 0; h < 2; ++h) {
+          const float (&v)[32] = acc[0][h];
+#pragma unroll
+          for (int j = 0; j < 32; j += 16) {
             uint4 q;
-            q.x = e4m3x4(acc0[16 * j] * f, acc0[16 * j + 1] * f, acc0[16 * j + 2] * f, acc0[16 * j + 3] * f);
-            q.y = e4m3x4(acc0[16 * j + 4] * f, acc0[16 * j + 5] * f, acc0[16 * j + 6] * f, acc0[16 * j + 7] * f);
-            q.z = e4m3x4(acc0[16 * j + 8] * f, acc0[16 * j + 9] * f, acc0[16 * j + 10] * f, acc0[16 * j + 11] * f);
-            q.w = e4m3x4(acc0[16 * j + 12] * f, acc0[16 * j + 13] * f, acc0[16 * j + 14] * f, acc0[16 * j + 15] * f);
-            dst[j] = q;
+            q.x = e4m3x4(v[j] * f, v[j + 1] * f, v[j + 2] * f, v[j + 3] * f);
+            q.y = e4m3x4(v[j + 4] * f, v[j + 5] * f, v[j + 6] * f, v[j + 7] * f);
+            q.z = e4m3x4(v[j + 8] * f, v[j + 9] * f, v[j + 10] * f, v[j + 11] * f);
+            q.w = e4m3x4(v[j + 12] * f, v[j + 13] * f, v[j + 14] * f, v[j + 15] * f);
+            *reinterpret_cast<uint4*>(buf_out + f8_unit(lane, 2 * h + j / 16)) = q;
           }
-          if (half == 0) a.hs[pos * f8_scale_pitch(a.n) + ni] = am / kE4m3Max;
         }
-      } else if (live) {
-        int64_t o;
-        if constexpr (MODE == kFp8Linear) o = static_cast<int64_t>(src) * a.out_stride;
-        else o = static_cast<int64_t>(slot / a.s) * a.out_stride + static_cast<int64_t>(slot % a.s) * a.out_stride_s;
-        const int c = nb0 * kFp8Block + half * 64;
-        f8_store64(a.out, o + c, acc0, c, a.n, a.out_dtype, a.out_vec);
-        f8_store64(a.out, o + c + kFp8Block, acc1, c + kFp8Block, a.n, a.out_dtype, a.out_vec);
+        __syncwarp();
+        // units 0, 1: this part's 32 of the low 64 columns, 2, 3: of the high ones; 8 rows at a time
+        uint8_t* dst = a.hq + static_cast<int64_t>(pos0 + warp_row) * f8_row_pitch(a.n) + ni * kFp8Block + part * 32 +
+                       ((lane & 3) >> 1) * 64 + (lane & 1) * 16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 8 * i + (lane >> 2);
+          if (warp_row + r < rows)
+            *reinterpret_cast<uint4*>(dst + r * f8_row_pitch(a.n)) =
+                *reinterpret_cast<const uint4*>(buf_out + f8_unit(r, lane & 3));
+        }
+        if (live && part == 0) a.hs[ni * a.scale_rows + pos0 + row] = am / kE4m3Max;
+      } else if (warp_live) {
+        int64_t o = -1;
+        if (live) {
+          if constexpr (MODE == kFp8Linear) {
+            o = static_cast<int64_t>(pos0 + row) * a.out_stride;
+          } else {
+            const int slot = __ldcg(a.sorted + pos0 + row);
+            o = static_cast<int64_t>(slot / a.s) * a.out_stride + static_cast<int64_t>(slot % a.s) * a.out_stride_s;
+          }
+        }
+        const int c = 2 * ni * kFp8Block + part * 32;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            f8_store32(a.out, o, acc[b][h], c + b * kFp8Block + h * 64, a.n, a.out_dtype, a.out_vec, buf_out);
       }
     }
   }
 
   __syncthreads();
-  if (*abort_flag && tid == 32 * kF8MmaWarp) {
-    tc_commit(drain);
-    mbar_wait_bounded(drain, 0);
-  }
-  if (*abort_flag && tid == 32 * kF8CopyWarp) {
-    const int issued = s_issued;  // copies: the latest use of each stage
-    for (int st = 0; st < kF8Stages && st < issued; ++st) {
-      const int last = st + ((issued - 1 - st) / kF8Stages) * kF8Stages;
-      mbar_wait_bounded(&full[st], (last / kF8Stages) & 1);
-    }
+  if (*abort_flag && tid == 0) {  // what is in flight gets 10 ms to end before the memory goes
+    const uint64_t t0 = global_ns();
+    while (global_ns() - t0 < 10000000ull) __nanosleep(1000);
   }
   tc_fence_before();
   __syncthreads();
+  f8_cluster_sync();  // neither CTA leaves while the other still uses its memory
   if (warp == kF8MmaWarp)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kF8TmemCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kF8TmemCols) : "memory");
 }
 
 // ---- what the products need first ------------------------------------------------------------
@@ -374,11 +591,18 @@ struct F8PrepArgs {
   const void* x;
   int64_t x_stride;
   int rows, k, x_vec;
-  uint8_t* xq;  // [rows][f8_row_pitch(k)], columns from k on zero
-  float* sx;    // [rows][f8_scale_pitch(k)]
+  uint8_t* xq;  // [rows or positions][f8_row_pitch(k)], columns from k on zero
+  float* sx;    // [blocks][scale_rows]
+  int64_t scale_rows;
+  const int* place;  // [rows][s] position of each slot, -1: not computed; NULL: a row is its own position
+  int s;
+  void* out;         // with place: rows of slots that are not computed are set to 0 (NULL: left alone)
+  int out_dtype, out_vec;
+  int64_t out_stride, out_stride_s;
 };
 
-// x's 8-bit form: 16 lanes a block of 128 columns, 8 columns a lane.
+// x's 8-bit form: 16 lanes a block of 128 columns, 8 columns a lane, kF8RowUnroll blocks at a time.
+constexpr int kF8RowUnroll = 4;
 template <typename TX>
 __global__ void __launch_bounds__(256) k_fp8_rows(F8PrepArgs a) {
   pdl_launch_dependents();
@@ -386,35 +610,159 @@ __global__ void __launch_bounds__(256) k_fp8_rows(F8PrepArgs a) {
   const int64_t n = static_cast<int64_t>(a.rows) * kb;
   const int sub = threadIdx.x & 15;
   const int64_t step = (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 4;
-  for (int64_t i0 = (static_cast<int64_t>(blockIdx.x) * blockDim.x + (threadIdx.x & ~31)) >> 4; i0 < n; i0 += step) {
-    const int64_t i = i0 + ((threadIdx.x >> 4) & 1);  // whole warps iterate together (shuffles)
-    const bool on = i < n;
-    const int64_t row = on ? i / kb : 0;
-    const int b = on ? static_cast<int>(i % kb) : 0;
-    const int c = b * kFp8Block + sub * 8;
-    const TX* src = static_cast<const TX*>(a.x) + row * a.x_stride;
-    float v[8];
-    if (on && a.x_vec && c + 8 <= a.k) {
-      load8<TX>(src + c, v);
-    } else {
+  if (a.place) pdl_wait();  // the plan
+  // whole warps iterate together (shuffles)
+  for (int64_t i0 = (static_cast<int64_t>(blockIdx.x) * blockDim.x + (threadIdx.x & ~31)) >> 4; i0 < n;
+       i0 += step * kF8RowUnroll) {
+    float v[kF8RowUnroll][8];
+    int row[kF8RowUnroll], b[kF8RowUnroll];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = on && c + j < a.k ? to_f32<TX>(src[c + j]) : 0.f;
+    for (int u = 0; u < kF8RowUnroll; ++u) {
+      const int64_t i = i0 + u * step + ((threadIdx.x >> 4) & 1);
+      row[u] = i < n ? static_cast<int>(i / kb) : -1;
+      b[u] = i < n ? static_cast<int>(i - static_cast<int64_t>(row[u]) * kb) : 0;
+      const int c = b[u] * kFp8Block + sub * 8;
+      const TX* src = static_cast<const TX*>(a.x) + static_cast<int64_t>(max(row[u], 0)) * a.x_stride;
+      if (row[u] >= 0 && a.x_vec && c + 8 <= a.k) {
+        load8<TX>(src + c, v[u]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[u][j] = row[u] >= 0 && c + j < a.k ? to_f32<TX>(src[c + j]) : 0.f;
+      }
     }
-    uint32_t m = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j]));
+    for (int u = 0; u < kF8RowUnroll; ++u) {
+      uint32_t m = 0;
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float am = fp8_amax(m);
-    const float f = kE4m3Max / am;
-    if (on) {
+      for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[u][j]));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      if (row[u] < 0) continue;
+      const float am = fp8_amax(m);
+      const float f = kE4m3Max / am, s = am / kE4m3Max;
       uint2 q;
-      q.x = e4m3x4(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
-      q.y = e4m3x4(v[4] * f, v[5] * f, v[6] * f, v[7] * f);
-      *reinterpret_cast<uint2*>(a.xq + row * f8_row_pitch(a.k) + c) = q;
-      if (sub == 0) a.sx[row * f8_scale_pitch(a.k) + b] = am / kE4m3Max;
+      q.x = e4m3x4(v[u][0] * f, v[u][1] * f, v[u][2] * f, v[u][3] * f);
+      q.y = e4m3x4(v[u][4] * f, v[u][5] * f, v[u][6] * f, v[u][7] * f);
+      const int c = b[u] * kFp8Block + sub * 8;
+      if (!a.place) {
+        *reinterpret_cast<uint2*>(a.xq + row[u] * f8_row_pitch(a.k) + c) = q;
+        if (sub == 0) a.sx[b[u] * a.scale_rows + row[u]] = s;
+        continue;
+      }
+      for (int t = 0; t < a.s; ++t) {
+        const int64_t p = a.place[static_cast<int64_t>(row[u]) * a.s + t];
+        if (p >= 0) {
+          *reinterpret_cast<uint2*>(a.xq + p * f8_row_pitch(a.k) + c) = q;
+          if (sub == 0) a.sx[b[u] * a.scale_rows + p] = s;
+        } else if (a.out) {
+          const int64_t o = row[u] * a.out_stride + t * a.out_stride_s + c;
+          if (a.out_vec && c + 8 <= a.k) {
+            const float z[8] = {};
+            if (a.out_dtype == ALUT_BF16) store8(static_cast<__nv_bfloat16*>(a.out) + o, z);
+            else if (a.out_dtype == ALUT_F16) store8(static_cast<__half*>(a.out) + o, z);
+            else store8(static_cast<float*>(a.out) + o, z);
+          } else {
+            for (int j = 0; j < 8; ++j)
+              if (c + j < a.k) store_any(a.out, o + j, 0.f, a.out_dtype);
+          }
+        }
+      }
     }
   }
+}
+
+// The plan: computed slots grouped by expert, by one cluster of CTAs that share the slots. Each
+// counts its share per expert in shared memory; after a cluster barrier every CTA knows the counts
+// before its own (distributed shared memory) and places its slots, in any order within an expert (a
+// row's result does not depend on its place). groups[i] = (expert, first position, rows <=
+// group_rows, 0). One CTA took 42 us for 32768 slots.
+constexpr int kF8PlanThreads = 1024;
+constexpr int kF8PlanCtas = 8;
+
+__global__ void __launch_bounds__(kF8PlanThreads) __cluster_dims__(kF8PlanCtas, 1, 1)
+    k_fp8_plan(Fp8Route r, int group_rows, int* sorted, int* place, int4* groups, int* n_groups) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  extern __shared__ int plan_smem[];
+  int* count = plan_smem;       // [E] this CTA's slots per expert
+  int* next = plan_smem + r.e;  // [E] next position
+  __shared__ int s_warp[32][2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = static_cast<int>(cluster.block_rank());
+  const int n = r.q * r.s;
+  const int step = kF8PlanThreads * kF8PlanCtas;
+  pdl_launch_dependents();
+  for (int e = tid; e < r.e; e += kF8PlanThreads) count[e] = 0;
+  __syncthreads();
+  bool bad = false;
+#pragma unroll 4
+  for (int64_t i = rank * kF8PlanThreads + tid; i < n; i += step) {
+    const int e = fp8_slot_expert(r, static_cast<int>(i), bad);
+    if (e >= 0) atomicAdd(&count[e], 1);
+  }
+  if (bad && r.err) atomicOr(r.err, static_cast<uint32_t>(kErrBadExpert));
+  cluster.sync();
+  // Exclusive prefix of (slots, groups) over the experts, two consecutive experts per thread.
+  int c[2], g[2], mine[2];  // mine: slots of the CTAs before this one
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int e = 2 * tid + j;
+    c[j] = mine[j] = 0;
+    if (e < r.e) {
+#pragma unroll
+      for (int k = 0; k < kF8PlanCtas; ++k) {
+        const int v = cluster.map_shared_rank(count, k)[e];
+        c[j] += v;
+        if (k < rank) mine[j] += v;
+      }
+    }
+    g[j] = (c[j] + group_rows - 1) / group_rows;
+  }
+  int sc = c[0] + c[1], sg = g[0] + g[1];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int pc = __shfl_up_sync(0xffffffffu, sc, o), pg = __shfl_up_sync(0xffffffffu, sg, o);
+    if (lane >= o) {
+      sc += pc;
+      sg += pg;
+    }
+  }
+  if (lane == 31) {
+    s_warp[warp][0] = sc;
+    s_warp[warp][1] = sg;
+  }
+  __syncthreads();
+  int bc = 0, bg = 0;
+  for (int w = 0; w < warp; ++w) {
+    bc += s_warp[w][0];
+    bg += s_warp[w][1];
+  }
+  int pos = bc + sc - c[0] - c[1], gi = bg + sg - g[0] - g[1];
+  if (rank == 0 && tid == kF8PlanThreads - 1) *n_groups = bg + sg;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int e = 2 * tid + j;
+    if (e < r.e) {
+      next[e] = pos + mine[j];
+      if (rank == 0)
+        for (int k = 0; k < g[j]; ++k)
+          groups[gi + k] = make_int4(e, pos + k * group_rows, min(group_rows, c[j] - k * group_rows), 0);
+    }
+    pos += c[j];
+    gi += g[j];
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int64_t i = rank * kF8PlanThreads + tid; i < n; i += step) {
+    const int e = fp8_slot_expert(r, static_cast<int>(i), bad);
+    int p = -1;
+    if (e >= 0) {
+      p = atomicAdd(&next[e], 1);
+      sorted[p] = static_cast<int>(i);
+    }
+    place[i] = p;
+  }
+  cluster.sync();  // no CTA leaves while another reads its counts
 }
 
 }  // namespace alut
