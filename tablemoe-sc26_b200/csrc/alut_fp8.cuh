@@ -159,20 +159,34 @@ constexpr int kFp8MaxExperts = 2048;  // two per thread of the plan
 // ---- the weight-streaming product ---------------------------------------------------------------
 //
 // For few rows per weight the time is the weights' way from HBM. A CTA takes 8 rows of x (the
-// N of mma.sync m16n8k32, weights as the M operand) and 32 weight rows: two 16-row tiles,
-// which are the gate and the up rows of 16 hidden units, or 32 adjacent output columns. Its
-// warps split K by blocks of 128 and add up through shared memory in warp order. Every
-// operand goes from global memory straight to registers: a lane reads 16 consecutive bytes of
-// its weight row (4 lanes a row, both 64-byte halves of a block), and since a dot product may
-// be taken in any order of k, those words are used as they come, x's in the same order; no
-// shared memory, no shuffle. x is quantised in registers by the warp that needs it: lane
-// (g, c) holds 32 of row g's 128 columns, four lanes agree on the maximum.
+// N of mma.sync m16n8k32, weights as the M operand) and a slice of weight rows, in steps of
+// two 16-row tiles per warp, which are the gate and the up rows of 16 hidden units, or 32 adjacent
+// output columns. The eight warps are 8 / ks row groups; the ks warps of a group split K by blocks of
+// 128 and add up through shared memory in warp order: ks = 8 where few CTAs have to hide the latency
+// of one token, less where there are enough (fewer barriers per byte).
+// The weights come by 16-byte asynchronous copies into a ring in shared memory, kStreamDepth steps
+// ahead: 64 KB in flight per CTA, two CTAs per SM, where registers held a quarter of that (and the
+// decode step of 128 experts took 194 us instead of DECODE_US). Every lane copies the 16 bytes that it
+// reads itself (4 lanes a row, both 64-byte halves of a block), so the ring needs no barrier; and
+// since a dot product may be taken in any order of k, those words are used as they lie, x's in the
+// same order. x is quantised once per CTA, by the warp that needs the block: lane (g, c) holds 32
+// of row g's 128 columns, four lanes agree on the maximum, the words wait in shared memory.
 // The slots of an expert are served 8 at a time; a group's first slot leads (no plan pass).
 
 constexpr int kStreamRows = 8;        // rows of x per CTA
-constexpr int kStreamWRows = 16;      // weight rows per tile, two tiles per CTA
-constexpr int kStreamMaxWarps = 8;
+constexpr int kStreamWRows = 16;      // weight rows per tile, two tiles per step
+constexpr int kStreamWarps = 8;
+constexpr int kStreamMaxSteps = 3;    // steps per CTA
 constexpr int kStreamMaxSlots = 512;  // slots a leader search looks through
+constexpr int kStreamMaxBlocks = 64;  // of 128 columns: x's words in shared memory take 1 KB each
+constexpr int kStreamDepth = 2;       // steps' weights in flight per warp
+constexpr int kStreamStepUnits = 8 * 32;  // 16-byte units of a warp's step: [tile][row g, g + 8][64-byte half][lane]
+// Shared memory: the ring [warps][depth][units], x's words [block][2][32 lanes] and scales
+// [block][8 rows], the weight's scales [steps][row group][tile][block].
+__host__ __device__ inline size_t stream_smem_bytes(int k, int steps, int ks) {
+  return static_cast<size_t>(kStreamWarps) * kStreamDepth * kStreamStepUnits * sizeof(uint4) +
+         static_cast<size_t>(fp8_blocks(k)) * (64 * sizeof(uint4) + (kStreamRows + 2 * steps * (kStreamWarps / ks)) * sizeof(float));
+}
 
 enum Fp8Mode { kFp8Linear = 0, kFp8GateUp = 1, kFp8Down = 2 };
 
@@ -189,31 +203,14 @@ struct StreamArgs {
   int out_dtype;
   int64_t out_stride, out_stride_s;
   int zero_skipped;
+  int steps, lks;           // steps per CTA, log2 of the warps that split K
 };
 
-__device__ __forceinline__ uint4 ldg_stream(const uint8_t* p) {  // read once: past L1
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
-// 16 bytes of a weight row from column c on, zero from column k on.
-__device__ __forceinline__ uint4 weight16(const uint8_t* row, int c, int k, bool live) {
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (live && c < k) {
-    v = ldg_stream(row + c);
-    if (c + 16 > k) {  // the row's last chunk: what pads the row is no data
-      uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int have = k - c - 4 * j;
-        if (have <= 0) w[j] = 0;
-        else if (have < 4) w[j] &= (1u << (8 * have)) - 1u;
-      }
-    }
-  }
-  return v;
+// 16 bytes to shared memory, of which the first `bytes` are read and the rest zero.
+__device__ __forceinline__ void cp_async16_part(void* dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+               "l"(src), "r"(bytes)
+               : "memory");
 }
 // 16 elements of a row of x from column c on, zero from column k on.
 // COHERENT: the rows were written by the kernel this one may overlap (not the read-only path).
@@ -254,13 +251,22 @@ __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
 template <typename TX, int MODE>
-__global__ void __launch_bounds__(32 * kStreamMaxWarps) k_fp8_stream(StreamArgs a) {
+__global__ void __launch_bounds__(32 * kStreamWarps, 2) k_fp8_stream(StreamArgs a) {
   constexpr unsigned kAll = 0xffffffffu;
-  __shared__ float red[kStreamMaxWarps][2][kStreamRows][kStreamWRows + 1];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nwarps = blockDim.x >> 5;
+  constexpr int kStepRows = MODE == kFp8GateUp ? kStreamWRows : 2 * kStreamWRows;  // of each half
+  extern __shared__ uint4 stream_smem[];
+  __shared__ float red[2][kStreamWarps][2][kStreamRows][kStreamWRows + 1];  // [parity of the step]
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int ks = 1 << a.lks, groups = kStreamWarps >> a.lks;  // of rows
+  const int ki = warp & (ks - 1), rg = warp >> a.lks;         // this warp's share of K, its row group
   const int g = lane >> 2, c = lane & 3;
   const int y = blockIdx.x;  // rows: CTAs that share weights run together
   const int slice = blockIdx.y;
+  const int kblocks = fp8_blocks(a.k), nblocks = fp8_blocks(a.n);
+  uint4* ring = stream_smem + warp * kStreamDepth * kStreamStepUnits + lane;
+  uint4* xw = stream_smem + kStreamWarps * kStreamDepth * kStreamStepUnits;  // [kblocks][2][32]
+  float* xs = reinterpret_cast<float*>(xw + kblocks * 64);              // [kblocks][8]
+  float* sws = xs + kblocks * kStreamRows;                              // [steps][groups][2][kblocks]
   pdl_launch_dependents();
   // This CTA's rows: lane m < cnt holds the m-th (Linear: row, otherwise slot).
   int cnt, member = 0, expert = 0;
@@ -268,134 +274,184 @@ __global__ void __launch_bounds__(32 * kStreamMaxWarps) k_fp8_stream(StreamArgs 
     cnt = min(kStreamRows, a.m - y * kStreamRows);
     member = y * kStreamRows + lane;
   } else {
+    const int n = a.r.q * a.r.s;
+    int ids[kStreamMaxSlots / 32];  // the slots' experts, all loads at once
     bool bad = false;
-    const int mine = fp8_slot_expert(a.r, y, bad);
-    if (bad && a.r.err && tid == 0 && slice == 0) atomicOr(a.r.err, static_cast<uint32_t>(kErrBadExpert));
+#pragma unroll
+    for (int i = 0; i < kStreamMaxSlots / 32; ++i) {
+      bool ignored = false;
+      ids[i] = 32 * i + lane < n ? fp8_slot_expert(a.r, 32 * i + lane, ignored) : -1;
+      bad |= ignored && 32 * i + lane == y;
+    }
+    if (bad && a.r.err && warp == 0 && slice == 0) atomicOr(a.r.err, static_cast<uint32_t>(kErrBadExpert));
+    int mine = -1;
+#pragma unroll
+    for (int i = 0; i < kStreamMaxSlots / 32; ++i)
+      if (i == y >> 5) mine = __shfl_sync(kAll, ids[i], y & 31);
     if (mine < 0) {
       if (MODE == kFp8Down && a.zero_skipped) {
         const int64_t o = static_cast<int64_t>(y / a.r.s) * a.out_stride + (y % a.r.s) * a.out_stride_s;
-        for (int i = tid; i < 2 * kStreamWRows; i += blockDim.x) {
-          const int col = slice * 2 * kStreamWRows + i;
-          if (col < a.n) store_any(a.out, o + col, 0.f, a.out_dtype);
-        }
+        const int c0 = slice * a.steps * groups * kStepRows, c1 = min(a.n, c0 + a.steps * groups * kStepRows);
+        for (int i = c0 + tid; i < c1; i += blockDim.x) store_any(a.out, o + i, 0.f, a.out_dtype);
       }
       return;
     }
     expert = mine;
-    const int n = a.r.q * a.r.s;
     int before = 0;
     cnt = 0;
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      bool ignored = false;
-      const bool same = i0 + lane < n && fp8_slot_expert(a.r, i0 + lane, ignored) == mine;
-      unsigned hits = __ballot_sync(kAll, same);
-      if (i0 <= y) {
-        const unsigned below = y - i0 < 32 ? (1u << (y - i0)) - 1u : kAll;
+#pragma unroll
+    for (int i = 0; i < kStreamMaxSlots / 32; ++i) {
+      unsigned hits = __ballot_sync(kAll, ids[i] == mine);
+      if (32 * i <= y) {
+        const unsigned below = y - 32 * i < 32 ? (1u << (y - 32 * i)) - 1u : kAll;
         before += __popc(hits & below);
         hits &= ~below;
       }
       while (hits && cnt < kStreamRows) {
         const int b = __ffs(hits) - 1;
         hits &= hits - 1;
-        if (lane == cnt) member = i0 + b;
+        if (lane == cnt) member = 32 * i + b;
         ++cnt;
       }
     }
     if (before % kStreamRows) return;
   }
-  const int r0 = slice * (MODE == kFp8GateUp ? kStreamWRows : 2 * kStreamWRows);
-  const int kblocks = fp8_blocks(a.k), nblocks = fp8_blocks(a.n);
-  const uint8_t* wrow[2];
-  const float* wscale[2];
-  bool lo_live[2], hi_live[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = r0 + (MODE == kFp8GateUp ? 0 : i * kStreamWRows);
-    const int half = MODE == kFp8GateUp ? i : 0;
-    wrow[i] = a.w + expert * a.w_stride_e + half * a.w_stride_half + static_cast<int64_t>(row + g) * a.w_stride;
-    wscale[i] = a.ws + ((static_cast<int64_t>(expert) * (MODE == kFp8GateUp ? 2 : 1) + half) * nblocks +
-                        min(row / kFp8Block, nblocks - 1)) * kblocks;
-    lo_live[i] = row + g < a.n;
-    hi_live[i] = row + g + 8 < a.n;
-  }
-  const int src = __shfl_sync(kAll, member, g);
-  const TX* xrow = static_cast<const TX*>(a.x) + static_cast<int64_t>(MODE == kFp8GateUp ? src / a.r.s : src) * a.x_stride;
-  const bool live = g < cnt;
-  float acc[2][4] = {};
-  bool waited = false;
-  for (int kb = warp; kb < kblocks; kb += nwarps) {
-    uint4 wv[2][2][2];  // [tile][half row][64-byte half]
-    const int c0 = kb * kFp8Block + 16 * c;
+  const int all = groups * kStepRows;  // rows of a step
+  const int r0 = slice * a.steps * all;
+  const int steps = min(a.steps, (a.n - r0 + all - 1) / all);
+  const int mykb = (kblocks - ki + ks - 1) >> a.lks;  // k-blocks ki, ki + ks, ...
+  const int row0 = r0 + rg * kStepRows;           // this warp's first rows
+  const uint8_t* wbase = a.w + expert * a.w_stride_e + static_cast<int64_t>(row0 + g) * a.w_stride + 16 * c;
+  const int64_t tile_stride = MODE == kFp8GateUp ? a.w_stride_half : kStreamWRows * a.w_stride;
+  // Every row and column of the slice is there: no copy needs to look.
+  const bool whole = (a.k & (kFp8Block - 1)) == 0 && r0 + steps * all <= a.n;
+  auto issue = [&](int step, int kb, int stage) {  // this warp's operands of one step
+    const uint8_t* p = wbase + static_cast<int64_t>(step) * all * a.w_stride + kb * kFp8Block;
+    uint4* dst = ring + stage * kStreamStepUnits;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        wv[i][0][j] = weight16(wrow[i], c0 + 64 * j, a.k, lo_live[i]);
-        wv[i][1][j] = weight16(wrow[i] + 8 * a.w_stride, c0 + 64 * j, a.k, hi_live[i]);
-      }
-    const float sw0 = wscale[0][kb], sw1 = wscale[1][kb];
-    if (MODE == kFp8Down && !waited) pdl_wait();  // the weights are on their way meanwhile
-    waited = true;
-    float xv[2][16];
-    x16<TX, MODE == kFp8Down>(xrow, c0, a.k, live, a.x_vec, xv[0]);
-    x16<TX, MODE == kFp8Down>(xrow, c0 + 64, a.k, live, a.x_vec, xv[1]);
-    uint32_t m = 0;
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) m = max(m, max(abs_bits(xv[0][j]), abs_bits(xv[1][j])));
-    m = max(m, __shfl_xor_sync(kAll, m, 1));
-    m = max(m, __shfl_xor_sync(kAll, m, 2));
-    const float am = fp8_amax(m);
-    const float f = kE4m3Max / am, sx = am / kE4m3Max;
-    const float sx0 = __shfl_sync(kAll, sx, 8 * c), sx1 = __shfl_sync(kAll, sx, 8 * c + 4);
-    float d[2][4] = {};
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      uint32_t xq[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        xq[i] = e4m3x4(xv[j][4 * i] * f, xv[j][4 * i + 1] * f, xv[j][4 * i + 2] * f, xv[j][4 * i + 3] * f);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        mma_e4m3(d[i], wv[i][0][j].x, wv[i][1][j].x, wv[i][0][j].y, wv[i][1][j].y, xq[0], xq[1]);
-        mma_e4m3(d[i], wv[i][0][j].z, wv[i][1][j].z, wv[i][0][j].w, wv[i][1][j].w, xq[2], xq[3]);
+        for (int j = 0; j < 2; ++j) {
+          const uint8_t* src = p + i * tile_stride + h * 8 * a.w_stride + 64 * j;
+          uint4* d = dst + (i * 4 + h * 2 + j) * 32;
+          if (whole) {
+            cp_async16(d, src);
+          } else {
+            const int row = row0 + step * all + (MODE == kFp8GateUp ? 0 : i * kStreamWRows) + 8 * h + g;
+            const int bytes = row < a.n ? max(0, min(16, a.k - (kb * kFp8Block + 16 * c + 64 * j))) : 0;
+            cp_async16_part(d, bytes > 0 ? src : a.w, bytes);
+          }
+        }
+  };
+  int istep = 0, ij = 0;  // the next to issue: for each step's rows, this warp's k-blocks
+  auto issue_next = [&](int stage) {
+    if (istep < steps) {
+      issue(istep, ki + ij * ks, stage);
+      if (++ij == mykb) {
+        ij = 0;
+        ++istep;
       }
     }
+    cp_async_commit();  // one group per step, empty behind the last
+  };
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float sw = i ? sw1 : sw0;
-      acc[i][0] = fmaf(d[i][0], sx0 * sw, acc[i][0]);
-      acc[i][1] = fmaf(d[i][1], sx1 * sw, acc[i][1]);
-      acc[i][2] = fmaf(d[i][2], sx0 * sw, acc[i][2]);
-      acc[i][3] = fmaf(d[i][3], sx1 * sw, acc[i][3]);
-    }
+  for (int i = 0; i < kStreamDepth; ++i) issue_next(i);
+  for (int st = warp; st < steps * groups * 2; st += kStreamWarps) {  // (step, row group, tile)
+    const int t = st & 1;
+    const int row = r0 + (st >> 1) * kStepRows + (MODE == kFp8GateUp ? 0 : t * kStreamWRows);
+    const int nb = min(row / kFp8Block, nblocks - 1);
+    const int64_t half = MODE == kFp8GateUp ? 2 * static_cast<int64_t>(expert) + t : expert;
+    for (int kb = lane; kb < kblocks; kb += 32) sws[st * kblocks + kb] = __ldg(a.ws + (half * nblocks + nb) * kblocks + kb);
   }
+  if constexpr (MODE == kFp8Down) pdl_wait();  // the weights are on their way meanwhile
+  {  // x's 8-bit form, a k-block per warp at a time
+    const int src = __shfl_sync(kAll, member, g);
+    const TX* xrow = static_cast<const TX*>(a.x) + static_cast<int64_t>(MODE == kFp8GateUp ? src / a.r.s : src) * a.x_stride;
+    const bool live = g < cnt;
+    for (int kb = warp; kb < kblocks; kb += kStreamWarps) {
+      const int c0 = kb * kFp8Block + 16 * c;
+      float xv[2][16];
+      x16<TX, MODE == kFp8Down>(xrow, c0, a.k, live, a.x_vec, xv[0]);
+      x16<TX, MODE == kFp8Down>(xrow, c0 + 64, a.k, live, a.x_vec, xv[1]);
+      uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    red[warp][i][2 * c][g] = acc[i][0];
-    red[warp][i][2 * c + 1][g] = acc[i][1];
-    red[warp][i][2 * c][g + 8] = acc[i][2];
-    red[warp][i][2 * c + 1][g + 8] = acc[i][3];
+      for (int j = 0; j < 16; ++j) m = max(m, max(abs_bits(xv[0][j]), abs_bits(xv[1][j])));
+      m = max(m, __shfl_xor_sync(kAll, m, 1));
+      m = max(m, __shfl_xor_sync(kAll, m, 2));
+      const float am = fp8_amax(m);
+      const float f = kE4m3Max / am;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          q[i] = e4m3x4(xv[j][4 * i] * f, xv[j][4 * i + 1] * f, xv[j][4 * i + 2] * f, xv[j][4 * i + 3] * f);
+        xw[(kb * 2 + j) * 32 + lane] = make_uint4(q[0], q[1], q[2], q[3]);
+      }
+      if (c == 0) xs[kb * kStreamRows + g] = am / kE4m3Max;
+    }
   }
   __syncthreads();
-  // Sums over the warps, 16 consecutive columns of a row by 16 consecutive threads. A warp
-  // handles whole rows, so that the member comes by a shuffle.
-  const int per = MODE == kFp8GateUp ? kStreamRows * kStreamWRows : 2 * kStreamRows * kStreamWRows;
-  for (int o = tid; o < per; o += blockDim.x) {  // per and blockDim.x are multiples of 32
-    const int col = o & 15, row = (o >> 4) & 7, i = o >> 7;
-    float v = 0.f, u = 0.f;
-    for (int w = 0; w < nwarps; ++w) {
-      v += red[w][MODE == kFp8GateUp ? 0 : i][row][col];
-      if (MODE == kFp8GateUp) u += red[w][1][row][col];
+  int stage = 0;
+  for (int step = 0; step < steps; ++step) {
+    float acc[2][4] = {};
+    for (int j = 0; j < mykb; ++j) {
+      const int kb = ki + j * ks;
+      cp_async_wait<kStreamDepth - 1>();
+      const uint4* w = ring + stage * kStreamStepUnits;
+      const uint4 x0 = xw[kb * 64 + lane], x1 = xw[kb * 64 + 32 + lane];
+      const float2 sx = *reinterpret_cast<const float2*>(xs + kb * kStreamRows + 2 * c);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint4 a0 = w[i * 128], a1 = w[i * 128 + 32], b0 = w[i * 128 + 64], b1 = w[i * 128 + 96];
+        float d[4] = {};
+        mma_e4m3(d, a0.x, b0.x, a0.y, b0.y, x0.x, x0.y);
+        mma_e4m3(d, a0.z, b0.z, a0.w, b0.w, x0.z, x0.w);
+        mma_e4m3(d, a1.x, b1.x, a1.y, b1.y, x1.x, x1.y);
+        mma_e4m3(d, a1.z, b1.z, a1.w, b1.w, x1.z, x1.w);
+        const float sw = sws[((step * groups + rg) * 2 + i) * kblocks + kb];
+        acc[i][0] = fmaf(d[0], sx.x * sw, acc[i][0]);
+        acc[i][1] = fmaf(d[1], sx.y * sw, acc[i][1]);
+        acc[i][2] = fmaf(d[2], sx.x * sw, acc[i][2]);
+        acc[i][3] = fmaf(d[3], sx.y * sw, acc[i][3]);
+      }
+      issue_next(stage);  // into the units just used
+      if (++stage == kStreamDepth) stage = 0;
     }
-    const int dst = __shfl_sync(kAll, member, row);
-    const int wr = r0 + (MODE == kFp8GateUp ? 0 : i * kStreamWRows) + col;
-    if (row >= cnt || wr >= a.n) continue;
-    if constexpr (MODE == kFp8GateUp) {
-      static_cast<float*>(a.out)[static_cast<int64_t>(dst) * a.out_stride + wr] = silu_mul(v, u);
-    } else if constexpr (MODE == kFp8Down) {
-      store_any(a.out, static_cast<int64_t>(dst / a.r.s) * a.out_stride + (dst % a.r.s) * a.out_stride_s + wr, v, a.out_dtype);
-    } else {
-      store_any(a.out, static_cast<int64_t>(dst) * a.out_stride + wr, v, a.out_dtype);
+    float(&part)[kStreamWarps][2][kStreamRows][kStreamWRows + 1] = red[step & 1];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      part[warp][i][2 * c][g] = acc[i][0];
+      part[warp][i][2 * c + 1][g] = acc[i][1];
+      part[warp][i][2 * c][g + 8] = acc[i][2];
+      part[warp][i][2 * c + 1][g + 8] = acc[i][3];
+    }
+    __syncthreads();  // (the step after next writes this half again, behind the next step's barrier)
+    // Sums over the warps, 16 consecutive columns of a row by 16 consecutive threads. A warp
+    // handles whole rows, so that the member comes by a shuffle.
+    // (16 rows of a row group's outputs: 8 rows of x, of one or two tiles; the absent are skipped.)
+    constexpr int kTiles = MODE == kFp8GateUp ? 1 : 2;
+    for (int o0 = warp * 32; o0 < groups * kTiles * kStreamRows * kStreamWRows; o0 += 32 * kStreamWarps) {
+      const int o = o0 + lane, col = o & 15;
+      const int row = (o >> 4) & 7, i = kTiles == 1 ? 0 : (o >> 7) & 1, og = kTiles == 1 ? o >> 7 : o >> 8;
+      const int dst = __shfl_sync(kAll, member, row);
+      const int wr = r0 + step * all + og * kStepRows + i * kStreamWRows + col;
+      if (row >= cnt || wr >= a.n) continue;
+      float v = 0.f, u = 0.f;
+      for (int w = og * ks; w < og * ks + ks; ++w) {
+        v += part[w][i][row][col];
+        if (MODE == kFp8GateUp) u += part[w][1][row][col];
+      }
+      if constexpr (MODE == kFp8GateUp) {
+        static_cast<float*>(a.out)[static_cast<int64_t>(dst) * a.out_stride + wr] = silu_mul(v, u);
+      } else if constexpr (MODE == kFp8Down) {
+        store_any(a.out, static_cast<int64_t>(dst / a.r.s) * a.out_stride + (dst % a.r.s) * a.out_stride_s + wr, v,
+                  a.out_dtype);
+      } else {
+        store_any(a.out, static_cast<int64_t>(dst) * a.out_stride + wr, v, a.out_dtype);
+      }
     }
   }
 }

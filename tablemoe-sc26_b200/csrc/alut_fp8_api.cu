@@ -27,22 +27,43 @@ static bool rows_vec(const void* x, int64_t stride, int dtype) {
 }
 
 template <int MODE>
-static int launch_stream(const StreamArgs& a, int x_dtype, unsigned groups, bool pdl, cudaStream_t st) {
-  const int rows = MODE == kFp8GateUp ? kStreamWRows : 2 * kStreamWRows;
-  const dim3 grid(groups, static_cast<unsigned>(ceil_div(a.n, rows)));
+static int launch_stream(StreamArgs a, int x_dtype, unsigned groups, bool pdl, cudaStream_t st) {
+  const int rows = MODE == kFp8GateUp ? kStreamWRows : 2 * kStreamWRows;  // of a row group
+  const int kblocks = fp8_blocks(a.k);
+  auto slices = [&](int ks, int steps) {
+    return static_cast<int64_t>(ceil_div(a.n, static_cast<int64_t>(steps) * (kStreamWarps / ks) * rows));
+  };
+  // Few CTAs: every warp a share of K, the shortest way through. Enough for two per SM: at least 3
+  // k-blocks a warp and up to kStreamMaxSteps steps per CTA, over which the search for the group and
+  // x's form are paid once.
+  a.steps = 1;
+  int ks = kStreamWarps;
+  while (ks > kblocks) ks /= 2;
+  int wide = ks;
+  while (wide > 1 && kblocks < 3 * wide) wide /= 2;
+  if (groups * slices(wide, 1) >= 2 * num_sms()) {
+    ks = wide;
+    while (a.steps < kStreamMaxSteps && groups * slices(wide, a.steps + 1) >= 4 * num_sms()) ++a.steps;
+  }
+  for (a.lks = 0; (1 << a.lks) < ks;) ++a.lks;
+  const dim3 grid(groups, static_cast<unsigned>(slices(ks, a.steps)));
   if (grid.y > 65535u) return fail(ALUT_ERANGE, "fp8: %d weight rows", a.n);
-  const dim3 block(32 * std::min(kStreamMaxWarps, fp8_blocks(a.k)));
+  const dim3 block(32 * kStreamWarps);
   void (*kern)(StreamArgs) = nullptr;
   if (MODE == kFp8Down || x_dtype == ALUT_F32) kern = k_fp8_stream<float, MODE>;
   if constexpr (MODE != kFp8Down) {
     if (x_dtype == ALUT_BF16) kern = k_fp8_stream<__nv_bfloat16, MODE>;
     if (x_dtype == ALUT_F16) kern = k_fp8_stream<__half, MODE>;
   }
+  const size_t smem = stream_smem_bytes(a.k, a.steps, ks);
+  // (with the kernel's static shared memory the default limit is reached below 48 KB)
+  const int rc = allow_smem(reinterpret_cast<const void*>(kern), std::max<size_t>(smem, 64 * 1024));
+  if (rc) return rc;
   if (!pdl) {
-    kern<<<grid, block, 0, st>>>(a);
+    kern<<<grid, block, smem, st>>>(a);
     return check_launch("k_fp8_stream");
   }
-  const cudaError_t e = launch_pdl(kern, grid, block, 0, st, a);
+  const cudaError_t e = launch_pdl(kern, grid, block, smem, st, a);
   if (e != cudaSuccess) return fail(ALUT_ECUDA, "k_fp8_stream: %s", cudaGetErrorString(e));
   return ALUT_OK;
 }
@@ -118,8 +139,10 @@ static int launch_rows(const F8PrepArgs& a, int x_dtype, cudaStream_t st) {
 }
 
 // Which product a call takes: the weight-streaming one below these row counts.
-static bool linear_streams(int m) { return m <= 16; }
-static bool experts_stream(int64_t slots) { return slots <= kStreamMaxSlots; }
+static bool linear_streams(int m, int k) { return m <= 16 && fp8_blocks(k) <= kStreamMaxBlocks; }
+static bool experts_stream(const alut_fp8_experts_t* ex, int64_t slots) {
+  return slots <= kStreamMaxSlots && fp8_blocks(std::max(ex->h, ex->i)) <= kStreamMaxBlocks;
+}
 
 struct LinearWorkspace {
   size_t xq, sx, total;
@@ -127,11 +150,11 @@ struct LinearWorkspace {
 static LinearWorkspace linear_layout(int m, int k) {
   LinearWorkspace w{};
   size_t off = 0;
-  if (!linear_streams(m)) {
+  if (!linear_streams(m, k)) {
     w.xq = off; off = align256(off + static_cast<size_t>(m) * f8_row_pitch(k));
     w.sx = off; off = align256(off + sizeof(float) * m * fp8_blocks(k));
   }
-  w.total = off + 256;
+  w.total = off;
   return w;
 }
 
@@ -144,7 +167,7 @@ static ExpertsWorkspace experts_layout(const alut_fp8_experts_t* ex, int q, int 
   ExpertsWorkspace w{};
   const int64_t n = static_cast<int64_t>(q) * s;
   size_t off = 0;
-  if (experts_stream(n)) {
+  if (experts_stream(ex, n)) {
     w.hidden = off; off = align256(off + sizeof(float) * n * round_up(ex->i, 4));
   } else {
     w.max_groups = ceil_div(n, kF8PairRows) + std::min<int64_t>(n, ex->num_experts);
@@ -223,10 +246,10 @@ int alut_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, int32_t x_dt
   int rc = check_weight("linear_fp8", w, w_scale, w_stride, k);
   if (rc) return rc;
   const size_t need = alut_linear_fp8_workspace_size(m, n, k);
-  if (!workspace || workspace_bytes < need)
+  if ((need && !workspace) || workspace_bytes < need)
     return fail(ALUT_EWORKSPACE, "linear_fp8: workspace has %zu bytes, needs %zu", workspace_bytes, need);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (!linear_streams(m)) {
+  if (!linear_streams(m, k)) {
     if (!aligned16(workspace)) return fail(ALUT_EWORKSPACE, "linear_fp8: workspace must be 16-byte aligned");
     const LinearWorkspace ws = linear_layout(m, k);
     char* base = static_cast<char*>(workspace);
@@ -304,7 +327,7 @@ int alut_experts_fp8(const alut_fp8_experts_t* ex, int32_t q, int32_t s, const v
   char* base = static_cast<char*>(workspace);
   const int n = q * s;
   Fp8Route r{q, s, ex->num_experts, sel, sel_stride, compute, compute_stride, error_bits};
-  if (!experts_stream(n)) {
+  if (!experts_stream(ex, n)) {
     F8PrepArgs p{};
     p.x = x;
     p.x_stride = x_stride;

@@ -41,33 +41,31 @@ def route_experts(router_logits, top_k, *, scoring="softmax", bias=None, n_group
     x = _check_logits(router_logits)
     q, e = x.shape
     dev = x.device
-    r = _alut.Router()
-    r.num_experts, r.top_k = e, int(top_k)
-    r.scoring = _choice(_SCORING, scoring, "scoring")
-    r.n_group = int(n_group)
-    r.topk_group = int(n_group if topk_group is None else topk_group)
-    r.group_rule = _choice(_GROUP_RULE, group_rule, "group_rule")
-    r.normalize_topk, r.scale = int(bool(normalize_topk)), float(scale)
-    if bias is not None:
-        if bias.shape != (e,) or bias.dtype != torch.float32 or bias.device != dev or not bias.is_contiguous():
-            raise ValueError(f"bias must be a contiguous fp32 tensor of shape ({e},) on {dev}")
-        r.bias = bias.data_ptr()
-    mode = _choice(_KEEP, keep, "keep")
-    if r.top_k <= 0:
+    top_k, n_group = int(top_k), int(n_group)
+    if top_k <= 0:
         raise ValueError(f"top_k must be positive, got {top_k}")
-    w = torch.empty(q, r.top_k, dtype=torch.float32, device=dev)
-    sel = torch.empty(q, r.top_k, dtype=torch.int64, device=dev)
-    masks = torch.empty(2, q, r.top_k, dtype=torch.bool, device=dev)
-    comp, reuse = masks[0], masks[1]
-    attn, ws = None, None
+    if bias is not None and (bias.shape != (e,) or bias.dtype != torch.float32 or bias.device != dev
+                             or not bias.is_contiguous()):
+        raise ValueError(f"bias must be a contiguous fp32 tensor of shape ({e},) on {dev}")
+    r = _alut.Router(e, top_k, _choice(_SCORING, scoring, "scoring"), n_group,
+                     n_group if topk_group is None else int(topk_group), _choice(_GROUP_RULE, group_rule, "group_rule"),
+                     1 if normalize_topk else 0, scale, None if bias is None else bias.data_ptr())
+    mode = _choice(_KEEP, keep, "keep")
+    shape = (q, top_k)
+    w = torch.empty(shape, dtype=torch.float32, device=dev)
+    sel = torch.empty(shape, dtype=torch.int64, device=dev)
+    comp = torch.empty(shape, dtype=torch.bool, device=dev)
+    reuse = torch.empty(shape, dtype=torch.bool, device=dev)
+    attn, ws, ws_bytes = None, None, 0
     if mode == 1:
         if attn_scores is not None and attn_scores.numel() == q:
             attn = attn_scores.reshape(-1).to(device=dev, dtype=torch.float32).contiguous()
         ws = _workspace(dev, e)
-    kk = -1 if keep_k is None else max(int(keep_k), 0)
-    rc = _alut.load().alut_route_experts(r, q, x.data_ptr(), _alut.dtype_code(x.dtype), x.stride(0), mode, kk,
-                                         float(keep_rate), _alut.ptr(attn), w.data_ptr(), sel.data_ptr(),
-                                         comp.data_ptr(), reuse.data_ptr(), r.top_k, _alut.ptr(ws),
-                                         0 if ws is None else ws.numel(), _alut.stream_ptr(dev))
-    _alut.check(rc, "alut_route_experts")
+        ws_bytes = ws.numel()
+    rc = _alut.load().alut_route_experts(r, q, x.data_ptr(), _alut.dtype_code(x.dtype), x.stride(0), mode,
+                                         -1 if keep_k is None else max(int(keep_k), 0), keep_rate, _alut.ptr(attn),
+                                         w.data_ptr(), sel.data_ptr(), comp.data_ptr(), reuse.data_ptr(), top_k,
+                                         _alut.ptr(ws), ws_bytes, _alut.stream_ptr(dev))
+    if rc:
+        _alut.check(rc, "alut_route_experts")
     return w, sel, comp, reuse

@@ -73,19 +73,21 @@ class _Fp8Module:
         self.device = device
         self._lib = _alut.load()
         self._errors = torch.zeros(1, dtype=torch.int32, device=device)
+        self._err = self._errors.data_ptr()
 
     def _check_x(self, x, width):
+        """x as rows (2D, unit innermost stride), its row stride and dtype code."""
         if x.device != self.device:
             raise ValueError(f"x is on {x.device}, the weights on {self.device}")
         if x.dim() < 1 or x.shape[-1] != width:
             raise ValueError(f"x must have {width} columns, got {tuple(x.shape)}")
-        x = x.reshape(-1, width)
-        if x.stride(-1) != 1 or x.stride(0) < width:  # also a broadcast row
+        if x.dim() != 2:
+            x = x.reshape(-1, width)
+        stride, inner = x.stride()
+        if inner != 1 or stride < width:  # also a broadcast row
             x = x.contiguous()
-        return x, _alut.dtype_code(x.dtype)
-
-    def _row_stride(self, x):
-        return max(x.stride(0), x.shape[-1])
+            stride = width
+        return x, stride, _alut.dtype_code(x.dtype)
 
     def device_errors(self, clear=True):
         """Error bits (ALUT_ERR_*) that this object's calls have set; waits for the current stream."""
@@ -94,9 +96,8 @@ class _Fp8Module:
             self._errors.zero_()
         return bits
 
-    def _finish(self, what):
-        if CacheConfig.ALUT_CHECK_ERRORS:
-            _alut.raise_device_errors(self.device_errors(), what)
+    def _raise_errors(self, what):
+        _alut.raise_device_errors(self.device_errors(), what)
 
 
 class Fp8Linear(_Fp8Module):
@@ -110,6 +111,7 @@ class Fp8Linear(_Fp8Module):
         self._init_device(weight.device)
         self.n, self.k = weight.shape
         self.weight, self.scale = _padded(weight), scale.contiguous()
+        self._w, self._w_stride, self._s = self.weight.data_ptr(), self.weight.stride(0), self.scale.data_ptr()
 
     @classmethod
     def quantize(cls, weight):
@@ -119,25 +121,27 @@ class Fp8Linear(_Fp8Module):
     def __call__(self, x, out=None, *, out_dtype=None):
         """x [..., K] (f32, bf16 or f16) -> [..., N] in ``out_dtype`` (default x's), or into ``out``
         (a 2D tensor [rows, N] with unit innermost stride)."""
-        v, xd = self._check_x(x, self.k)
-        m = v.shape[0]
+        v, xs, xd = self._check_x(x, self.k)
+        m, n, k = v.shape[0], self.n, self.k
         if out is None:
-            y = torch.empty(*x.shape[:-1], self.n, dtype=out_dtype or x.dtype, device=x.device)
-            stride = self.n
+            y = torch.empty((*x.shape[:-1], n), dtype=out_dtype or x.dtype, device=self.device)
+            stride = n
         else:
-            if out.shape != (m, self.n) or out.device != x.device or out.stride(-1) != 1:
-                raise ValueError(f"out must be a [{m}, {self.n}] tensor on {x.device} with unit innermost stride")
+            if out.shape != (m, n) or out.device != x.device or out.stride(-1) != 1:
+                raise ValueError(f"out must be a [{m}, {n}] tensor on {x.device} with unit innermost stride")
             if out_dtype is not None and out_dtype != out.dtype:
                 raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
-            y, stride = out, out.stride(0) if m > 1 else max(out.stride(0), self.n)
-        n = int(self._lib.alut_linear_fp8_workspace_size(m, self.n, self.k))
-        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-        rc = self._lib.alut_linear_fp8(m, self.n, self.k, v.data_ptr(), xd, self._row_stride(v), self.weight.data_ptr(),
-                                       self.weight.stride(0), self.scale.data_ptr(), y.data_ptr(),
-                                       _alut.dtype_code(y.dtype), stride, self._errors.data_ptr(), ws.data_ptr(), n,
-                                       _alut.stream_ptr(x.device))
-        _alut.check(rc, "alut_linear_fp8")
-        self._finish("alut_linear_fp8")
+            y, stride = out, out.stride(0) if m > 1 else max(out.stride(0), n)
+        lib = self._lib
+        nbytes = lib.alut_linear_fp8_workspace_size(m, n, k)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+        rc = lib.alut_linear_fp8(m, n, k, v.data_ptr(), xd, xs, self._w, self._w_stride, self._s, y.data_ptr(),
+                                 _alut.dtype_code(y.dtype), stride, self._err, _alut.ptr(ws), nbytes,
+                                 _alut.stream_ptr(self.device))
+        if rc:
+            _alut.check(rc, "alut_linear_fp8")
+        if CacheConfig.ALUT_CHECK_ERRORS:
+            self._raise_errors("alut_linear_fp8")
         return y
 
 
@@ -177,34 +181,38 @@ class Fp8Experts(_Fp8Module):
         the slots of ``compute_mask`` [Q, S] (None: all). Without ``collected`` a new tensor of x's
         dtype, 0 at the other slots; otherwise written into it (f32, bf16 or f16, unit innermost
         stride), its other rows untouched: the form of ``ALUTCachedMoE``'s ``run_experts``."""
-        v, xd = self._check_x(x, self.hidden)
-        if selected_experts.dim() != 2 or selected_experts.shape[0] != v.shape[0]:
-            raise ValueError(f"selected_experts must be [{v.shape[0]}, S], got {tuple(selected_experts.shape)}")
-        if selected_experts.dtype != torch.int64 or selected_experts.device != x.device:
+        v, xs, xd = self._check_x(x, self.hidden)
+        dev, h, sel = self.device, self.hidden, selected_experts
+        if sel.dim() != 2 or sel.shape[0] != v.shape[0]:
+            raise ValueError(f"selected_experts must be [{v.shape[0]}, S], got {tuple(sel.shape)}")
+        if sel.dtype != torch.int64 or sel.device != dev:
             raise ValueError("selected_experts must be int64 on x's device")
-        q, s = selected_experts.shape
-        sel = selected_experts if selected_experts.stride(-1) == 1 else selected_experts.contiguous()
-        comp = None
-        if compute_mask is not None:
-            if compute_mask.shape != (q, s) or compute_mask.dtype not in (torch.bool, torch.uint8) \
-                    or compute_mask.device != x.device:
+        q, s = sel.shape
+        sel_stride, inner = sel.stride()
+        if inner != 1 or sel_stride < s:
+            sel, sel_stride = sel.contiguous(), s
+        comp, comp_stride = compute_mask, s
+        if comp is not None:
+            if comp.shape != (q, s) or comp.dtype not in (torch.bool, torch.uint8) or comp.device != dev:
                 raise ValueError(f"compute_mask must be bool [{q}, {s}] on x's device")
-            comp = compute_mask if compute_mask.stride(-1) == 1 and compute_mask.stride(0) >= s \
-                else compute_mask.contiguous()
-        if sel.stride(0) < s:
-            sel = sel.contiguous()
+            comp_stride, inner = comp.stride()
+            if inner != 1 or comp_stride < s:
+                comp, comp_stride = comp.contiguous(), s
         out = collected
         if out is None:
-            out = torch.empty(q, s, self.hidden, dtype=x.dtype, device=x.device)
-        elif out.shape != (q, s, self.hidden) or out.device != x.device or out.stride(-1) != 1:
-            raise ValueError(f"collected must be [{q}, {s}, {self.hidden}] on {x.device} with unit innermost stride")
-        n = int(self._lib.alut_experts_fp8_workspace_size(self._weights, q, s))
-        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-        rc = self._lib.alut_experts_fp8(self._weights, q, s, v.data_ptr(), xd, self._row_stride(v), sel.data_ptr(),
-                                        max(sel.stride(0), s), _alut.ptr(comp), s if comp is None else max(comp.stride(0), s),
-                                        int(collected is None), out.data_ptr(), _alut.dtype_code(out.dtype), out.stride(0),
-                                        out.stride(1), self._errors.data_ptr(), ws.data_ptr(), n,
-                                        _alut.stream_ptr(x.device))
-        _alut.check(rc, "alut_experts_fp8")
-        self._finish("alut_experts_fp8")
+            out = torch.empty((q, s, h), dtype=x.dtype, device=dev)
+        elif out.shape != (q, s, h) or out.device != dev or out.stride(-1) != 1:
+            raise ValueError(f"collected must be [{q}, {s}, {h}] on {dev} with unit innermost stride")
+        out_t, out_s, _ = out.stride()
+        lib = self._lib
+        nbytes = lib.alut_experts_fp8_workspace_size(self._weights, q, s)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        rc = lib.alut_experts_fp8(self._weights, q, s, v.data_ptr(), xd, xs, sel.data_ptr(), sel_stride, _alut.ptr(comp),
+                                  comp_stride, 1 if collected is None else 0, out.data_ptr(),
+                                  _alut.dtype_code(out.dtype), out_t, out_s, self._err, ws.data_ptr(), nbytes,
+                                  _alut.stream_ptr(dev))
+        if rc:
+            _alut.check(rc, "alut_experts_fp8")
+        if CacheConfig.ALUT_CHECK_ERRORS:
+            self._raise_errors("alut_experts_fp8")
         return out

@@ -61,8 +61,8 @@ def test_linear_arguments():
     assert code(linear(w=PTR + 8), "16-byte") == _alut.ALUT_ESHAPE
     assert code(linear(wstride=40), "16-byte") == _alut.ALUT_ESHAPE
     assert code(linear(wstride=32), "< 48") == _alut.ALUT_ESHAPE
-    assert code(linear(nbytes=16), "workspace") == _alut.ALUT_EWORKSPACE
-    assert code(linear(work=None), "workspace") == _alut.ALUT_EWORKSPACE
+    assert code(linear(m=300, nbytes=16), "workspace") == _alut.ALUT_EWORKSPACE
+    assert code(linear(m=300, work=None), "workspace") == _alut.ALUT_EWORKSPACE
     assert linear(m=0, x=None) == _alut.ALUT_OK
     assert _alut.load().alut_linear_fp8_workspace_size(4, 0, 8) == 0
 
