@@ -116,10 +116,10 @@ static int encode_weight(CUtensorMap* map, const void* p, int k, int rows, int h
 template <int MODE>
 static int launch_tc(const CUtensorMap& xm, const CUtensorMap& wm, const F8Args& a, int64_t max_tiles, cudaStream_t st) {
   auto kern = k_fp8_tc<MODE>;
-  const int rc = allow_smem(reinterpret_cast<const void*>(kern), kF8SmemBytes);
+  const int rc = allow_smem(reinterpret_cast<const void*>(kern), f8_smem_bytes<MODE>);
   if (rc) return rc;
   const unsigned grid = 2 * static_cast<unsigned>(std::min<int64_t>(max_tiles, num_sms() / 2));  // pairs of CTAs
-  const cudaError_t e = launch_pdl(kern, dim3(grid), dim3(kF8Threads), kF8SmemBytes, st, xm, wm, a);
+  const cudaError_t e = launch_pdl(kern, dim3(grid), dim3(kF8Threads), f8_smem_bytes<MODE>, st, xm, wm, a);
   if (e != cudaSuccess) return fail(ALUT_ECUDA, "k_fp8_tc: %s", cudaGetErrorString(e));
   return ALUT_OK;
 }

@@ -15,7 +15,8 @@
 // issue, and reading it back (128 KB per SM through the TMEM port) takes 540. With two accumulators
 // of a whole k-block that chain ran at 1000 cycles a k-block.
 //
-//   warps 0-7  epilogue: TMEM lane quarter warp % 4, columns 32 (warp / 4) .. + 32 of each 64
+//   warps 0-7  epilogue: TMEM lane quarter warp % 4; part warp / 4 has half the columns: GateUp 32 of
+//              the gate's 64 and the same 32 of the up's, otherwise one of the two weight blocks
 //   warp 8     TMA copies (128-byte swizzle), signalled to the leader CTA's barrier
 //   warp 9     MMA issuer (of the pair's leader, rank 0)
 //   warp 10    the factors sx sw of a k-block's 128 rows and two blocks, into a ring in shared
@@ -25,6 +26,9 @@
 //   barriers:  full/empty per stage, full/empty per accumulator, full/empty per ring slot; the
 //              stages' full and the accumulators' empty count in the leader, the commits arrive in
 //              both CTAs
+// Linear and Down end with a row segment of 128 outputs per thread, written to shared memory and from
+// there by one bulk copy per row, which runs on while the next tile is added up (with store
+// instructions a tile's end took 4000 cycles: a fifth of the whole product of 8192 x 4096 outputs).
 // GateUp ends with h = silu(gate) * up, its 8-bit form (the 128 hidden units of the tile are one
 // block of the next product; the two column halves exchange their maxima) written for Down.
 // x's rows lie in the order of the plan (k_fp8_rows writes a token's 8-bit row once per computed
@@ -45,7 +49,10 @@ namespace alut {
 
 constexpr int kF8Rows = 128;                // rows of x per CTA
 constexpr int kF8PairRows = 2 * kF8Rows;    // per pair of CTAs
-constexpr int kF8Stages = 6;
+// Stages of copies: as many as the memory beside the output rows holds.
+template <int MODE>
+constexpr int f8_stages = MODE == 1 /* kFp8GateUp */ ? 6 : 4;
+constexpr int kF8MaxStages = 6;
 constexpr uint32_t kF8TileBytes = kF8Rows * kFp8Block;  // one 128 x 128 operand tile
 constexpr uint32_t kF8StageBytes = 2 * kF8TileBytes;    // x's rows, a weight block
 constexpr int kF8EpiWarps = 8;
@@ -55,11 +62,14 @@ constexpr int kF8Threads = 32 * (kF8EpiWarps + 4);
 constexpr int kF8EpiRegs = 232, kF8RoleRegs = 40;
 constexpr int kF8CopyWarp = kF8EpiWarps, kF8MmaWarp = kF8EpiWarps + 1, kF8ScaleWarp = kF8EpiWarps + 2, kF8WaitWarp = kF8EpiWarps + 3;
 constexpr int kF8Group = 4, kF8Ring = 2;     // factors of 4 k-blocks per ring slot
-constexpr uint32_t kF8StoreBytes = 32 * 64;  // a warp's output rows on their way out
+constexpr uint32_t kF8RowBytes = 256 + 16;    // an output row on its way out (padded: no bank conflicts)
+template <int MODE>  // a warp's 32 of them; GateUp: 32 x 64 bytes
+constexpr uint32_t f8_store_bytes = MODE == 1 ? 32 * 64 : 32 * kF8RowBytes;
 constexpr uint32_t kF8TmemCols = 512;
 constexpr int kF8Acc = 4, kF8AccCols = 128;  // accumulators
-constexpr size_t kF8SmemBytes = 1024 + 1024 + static_cast<size_t>(kF8Stages) * kF8StageBytes +
-                                kF8EpiWarps * kF8StoreBytes + kF8Ring * kF8Group * kF8Rows * sizeof(float2);
+template <int MODE>
+constexpr size_t f8_smem_bytes = 1024 + 1024 + static_cast<size_t>(f8_stages<MODE>) * kF8StageBytes +
+                                 kF8EpiWarps * f8_store_bytes<MODE> + kF8Ring * kF8Group * kF8Rows * sizeof(float2);
 
 // Scales of x's rows (and of the hidden rows) are kept [block][row]: a k-block's are adjacent.
 __host__ __device__ inline int64_t f8_row_pitch(int k) { return static_cast<int64_t>(fp8_blocks(k)) * kFp8Block; }
@@ -146,23 +156,49 @@ __device__ __forceinline__ void f8_load_weight(void* dst, const CUtensorMap* map
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(half), "r"(e), "r"(bar)
       : "memory");
 }
-__device__ __forceinline__ void f8_commit(uint64_t* bar) {  // arrives on `bar` of both CTAs
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-          smem_addr(bar)),
-      "h"(static_cast<uint16_t>(3))
-      : "memory");
-}
 // kind::f8f6f4 instruction descriptor: fp32 D, e4m3 A and B, K-major, M = 256, N = 128.
 __host__ __device__ __forceinline__ uint32_t f8_idesc() {
   return (1u << 4) | (static_cast<uint32_t>(kF8AccCols >> 3) << 17) | (static_cast<uint32_t>(kF8PairRows >> 4) << 24);
 }
-__device__ __forceinline__ void f8_mma(uint32_t tmem, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(
-          tmem),
-      "l"(da), "l"(db), "r"(idesc), "r"(acc)
-      : "memory");
+// One accumulator of a k-block: 4 MMAs of K = 32 (descriptors advance by 32 bytes), then the commits
+// that arrive in both CTAs: on `done`, and (LAST) on `freed`, the stage. A whole warp executes it and
+// one elected lane issues; the election, the predicate and the operands (uniform registers) stay in
+// one statement: as single instructions behind a branch the issue took 210 cycles a half k-block.
+template <bool LAST>
+__device__ __forceinline__ void f8_issue(uint32_t tmem, uint64_t dx, uint64_t dw, uint32_t idesc, uint32_t done,
+                                         uint32_t freed) {
+  if constexpr (LAST) {
+    asm volatile(
+        "{\n .reg .pred q, no, yes;\n .reg .b64 x, w;\n elect.sync _|q, 0xffffffff;\n"
+        " setp.ne.b32 no, 0, 0;\n setp.eq.b32 yes, 0, 0;\n"
+        " @q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, no;\n"
+        " add.u64 x, %1, 2;\n add.u64 w, %2, 2;\n"
+        " @q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], x, w, %3, yes;\n"
+        " add.u64 x, %1, 4;\n add.u64 w, %2, 4;\n"
+        " @q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], x, w, %3, yes;\n"
+        " add.u64 x, %1, 6;\n add.u64 w, %2, 6;\n"
+        " @q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], x, w, %3, yes;\n"
+        " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%4], %6;\n"
+        " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%5], %6;\n"
+        "}\n" ::"r"(tmem),
+        "l"(dx), "l"(dw), "r"(idesc), "r"(done), "r"(freed), "h"(static_cast<uint16_t>(3))
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n .reg .pred q, no, yes;\n .reg .b64 x, w;\n elect.sync _|q, 0xffffffff;\n"
+        " setp.ne.b32 no, 0, 0;\n setp.eq.b32 yes, 0, 0;\n"
+        " @q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, no;\n"
+        " add.u64 x, %1, 2;\n add.u64 w, %2, 2;\n"
+        " @q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], x, w, %3, yes;\n"
+        " add.u64 x, %1, 4;\n add.u64 w, %2, 4;\n"
+        " @q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], x, w, %3, yes;\n"
+        " add.u64 x, %1, 6;\n add.u64 w, %2, 6;\n"
+        " @q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], x, w, %3, yes;\n"
+        " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%4], %6;\n"
+        "}\n" ::"r"(tmem),
+        "l"(dx), "l"(dw), "r"(idesc), "r"(done), "r"(freed), "h"(static_cast<uint16_t>(3))
+        : "memory");
+  }
 }
 
 // 32 columns of this warp's 32 TMEM lanes, not waited for: the registers hold them after f8_ld_wait.
@@ -200,66 +236,81 @@ __device__ __forceinline__ uint32_t f8_unit(int r, int c) {
   return static_cast<uint32_t>(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
 }
 
-// A warp's 32 rows x C columns (lane r has row r's values v and its output offset o, negative for
-// no row) out through shared memory, so that a store instruction writes 64 adjacent bytes of 8 rows
-// (a row per thread writes 32 half sectors at a time).
+// Output rows. A thread has 64 or 128 columns (from c0 on) of its row (offset o; negative: no row):
+// into its own padded row of the warp's buffer, then one bulk copy of the row segment.
+__device__ __forceinline__ void f8_rows_reusable() {  // this thread's copies have read their rows
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
 template <typename TO, int C>
-__device__ __forceinline__ void f8_store(TO* out, int64_t o, const float* v, int c0, int n, bool vec, unsigned char* buf) {
-  static_assert(C * sizeof(TO) == 64, "a buffer row");
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ void f8_store_row(TO* out, int64_t o, const float (&v)[C], int c0, int n, bool vec,
+                                             unsigned char* rows) {
+  static_assert(C * sizeof(TO) == 256, "a buffer row");
   constexpr int kPer = 16 / sizeof(TO);
-  __syncwarp();
+  const int lane = threadIdx.x & 31;
+  unsigned char* mine = rows + lane * kF8RowBytes;
+  f8_rows_reusable();
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
+  for (int c = 0; c < C; c += kPer) {
     __align__(16) TO t[kPer];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) t[j] = from_f32<TO>(v[c * kPer + j]);
-    *reinterpret_cast<uint4*>(buf + f8_unit(lane, c)) = *reinterpret_cast<const uint4*>(t);
+    for (int j = 0; j < kPer; ++j) t[j] = from_f32<TO>(v[c + j]);
+    *reinterpret_cast<uint4*>(mine + c * sizeof(TO)) = *reinterpret_cast<const uint4*>(t);
   }
-  __syncwarp();
-  if (vec && c0 + C <= n) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 8 * i + (lane >> 2);
-      const int64_t ro = __shfl_sync(0xffffffffu, o, r);
-      const uint4 u = *reinterpret_cast<const uint4*>(buf + f8_unit(r, lane & 3));
-      if (ro >= 0) *reinterpret_cast<uint4*>(out + ro + c0 + (lane & 3) * kPer) = u;
-    }
-  } else {  // a ragged edge, or rows that do not start on 16 bytes: element by element along the row
+  const int have = min(C, n - c0);  // may be <= 0
+  if (vec && have % kPer == 0) {
+    fence_async_shared();
+    if (o >= 0 && have > 0)
+      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(out + o + c0), "r"(smem_addr(mine)),
+                   "r"(have * static_cast<int>(sizeof(TO)))
+                   : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  } else {  // a ragged edge, or rows that do not start on 16 bytes: element by element along the rows
+    __syncwarp();
     for (int r = 0; r < 32; ++r) {
       const int64_t ro = __shfl_sync(0xffffffffu, o, r);
-      if (ro >= 0 && lane < C && c0 + lane < n)
-        out[ro + c0 + lane] = *reinterpret_cast<const TO*>(buf + f8_unit(r, lane / kPer) + (lane % kPer) * sizeof(TO));
+      if (ro < 0) continue;
+      for (int c = lane; c < have; c += 32)
+        out[ro + c0 + c] = *reinterpret_cast<const TO*>(rows + r * kF8RowBytes + c * sizeof(TO));
     }
+    __syncwarp();
   }
 }
-__device__ __forceinline__ void f8_store32(void* out, int64_t o, const float (&v)[32], int c, int n, int dtype, bool vec,
-                                           unsigned char* buf) {
+// acc[i][h][j]: column c0 + 64 h + 32 i + j.
+__device__ __forceinline__ void f8_store_rows(void* out, int64_t o, const float (&acc)[2][2][32], int c0, int n, int dtype,
+                                              bool vec, unsigned char* rows) {
+  float v[128];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[64 * h + 32 * i + j] = acc[i][h][j];
   if (dtype == ALUT_BF16) {
-    f8_store<__nv_bfloat16, 32>(static_cast<__nv_bfloat16*>(out), o, v, c, n, vec, buf);
+    f8_store_row(static_cast<__nv_bfloat16*>(out), o, v, c0, n, vec, rows);
   } else if (dtype == ALUT_F16) {
-    f8_store<__half, 32>(static_cast<__half*>(out), o, v, c, n, vec, buf);
+    f8_store_row(static_cast<__half*>(out), o, v, c0, n, vec, rows);
   } else {
-    f8_store<float, 16>(static_cast<float*>(out), o, v, c, n, vec, buf);
-    f8_store<float, 16>(static_cast<float*>(out), o, v + 16, c + 16, n, vec, buf);
+    f8_store_row(static_cast<float*>(out), o, reinterpret_cast<const float (&)[64]>(v[0]), c0, n, vec, rows);
+    f8_store_row(static_cast<float*>(out), o, reinterpret_cast<const float (&)[64]>(v[64]), c0 + 64, n, vec, rows);
   }
 }
 
 template <int MODE>
 __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
     k_fp8_tc(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, F8Args a) {
+  constexpr int kStages = f8_stages<MODE>;
   extern __shared__ unsigned char f8_raw[];
   unsigned char* f8_smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(f8_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(f8_smem);  // [kF8Stages] (the leader's counts for the pair)
-  uint64_t* empty = full + kF8Stages;                     // [kF8Stages]
-  uint64_t* t_full = empty + kF8Stages;                   // [kF8Acc]
+  uint64_t* full = reinterpret_cast<uint64_t*>(f8_smem);  // [kStages] (the leader's counts for the pair)
+  uint64_t* empty = full + kF8MaxStages;                  // [kStages]
+  uint64_t* t_full = empty + kF8MaxStages;                  // [kF8Acc]
   uint64_t* t_empty = t_full + kF8Acc;                    // [kF8Acc] (the leader's counts for the pair)
   uint64_t* maxima = t_empty + kF8Acc;                    // [1] both column parts' maxima are there
   uint64_t* f_full = maxima + 1;                          // [kF8Ring]
   uint64_t* f_empty = f_full + kF8Ring;                   // [kF8Ring]
-  unsigned char* stages = f8_smem + 1024;                 // [kF8Stages][x rows | weight block]
-  unsigned char* out_buf = stages + kF8Stages * static_cast<size_t>(kF8StageBytes);  // [kF8EpiWarps][kF8StoreBytes]
-  float2* ring = reinterpret_cast<float2*>(out_buf + kF8EpiWarps * kF8StoreBytes);    // [kF8Ring][kF8Group][kF8Rows]
+  unsigned char* stages = f8_smem + 1024;                 // [kStages][x rows | weight block]
+  float2* ring = reinterpret_cast<float2*>(stages + kStages * static_cast<size_t>(kF8StageBytes));  // [kF8Ring][kF8Group][kF8Rows]
+  unsigned char* out_buf = reinterpret_cast<unsigned char*>(ring + kF8Ring * kF8Group * kF8Rows);    // output rows of 8 warps
   __shared__ float s_max[2][2][kF8Rows];                  // [tile parity][column half][row]
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
@@ -276,7 +327,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   if (tid == 0) {
-    for (int i = 0; i < kF8Stages; ++i) {
+    for (int i = 0; i < kStages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
@@ -326,7 +377,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
         const int wrow = MODE == kFp8GateUp ? ni * kFp8Block : (2 * ni + static_cast<int>(rank)) * kFp8Block;
         const int half = MODE == kFp8GateUp ? static_cast<int>(rank) : 0;
         const int xrow = g.y + static_cast<int>(rank) * kF8Rows;
-        for (int kb = 0; kb < kblocks; ++kb, (++st == kF8Stages ? (st = 0, past ^= 1) : 0)) {
+        for (int kb = 0; kb < kblocks; ++kb, (++st == kStages ? (st = 0, past ^= 1) : 0)) {
           wait(empty, st, past);
           if (f8_elect()) {
             unsigned char* sx = stages + static_cast<size_t>(st) * kF8StageBytes;
@@ -342,6 +393,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
       // ---- MMA issuer ----------------------------------------------------------------------------
       if (rank == 0) {
         int st = 0, ph = 0, buf = 0, past = 1;
+        const uint32_t done0 = smem_addr(t_full), freed0 = smem_addr(empty);
         const uint32_t idesc = f8_idesc();
         const uint64_t desc0 = pt_desc_sw128(smem_addr(stages));  // + address / 16 within the first 14 bits
         for (int64_t tile = pair; tile < ntiles && !stopped(); tile += npairs) {
@@ -352,18 +404,12 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
               const int acc = 2 * buf + h;
               wait(t_empty, acc, past);
               tc_fence_after();
-              if (f8_elect()) {
-                const uint64_t dx = desc0 + static_cast<uint32_t>(st) * (kF8StageBytes >> 4);
-                const uint64_t dw = dx + ((kF8TileBytes + h * kF8TileBytes / 2) >> 4);
-#pragma unroll
-                for (int k32 = 0; k32 < kFp8Block / 32; ++k32)
-                  f8_mma(tmem + acc * kF8AccCols, dx + 2 * k32, dw + 2 * k32, idesc, k32 ? 1u : 0u);
-                f8_commit(&t_full[acc]);
-                if (h) f8_commit(&empty[st]);
-              }
-              __syncwarp();
+              const uint64_t dx = desc0 + static_cast<uint32_t>(st) * (kF8StageBytes >> 4);
+              const uint64_t dw = dx + ((kF8TileBytes + h * kF8TileBytes / 2) >> 4);
+              if (h) f8_issue<true>(tmem + acc * kF8AccCols, dx, dw, idesc, done0 + 8 * acc, freed0 + 8 * st);
+              else f8_issue<false>(tmem + acc * kF8AccCols, dx, dw, idesc, done0 + 8 * acc, 0);
             }
-            if (++st == kF8Stages) {
+            if (++st == kStages) {
               st = 0;
               ph ^= 1;
             }
@@ -410,37 +456,47 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
       // ---- accumulators (and their factors) done: let the epilogue go ------------------------------
       // It and the epilogue run through every tile even after an abort, without waiting then: a
       // named barrier's counts have to match.
+      // The factors of k-block kb + 1 are there when the epilogue passes the barrier of (kb, 1).
       int sl = 0, sph = 0, buf = 0, ph = 0;
-      for (int64_t tile = pair; tile < ntiles; tile += npairs)
+      auto factors = [&](int kb) {
+        if (kb & (kF8Group - 1)) return;
+        if (!*abort_flag) wait(f_full, sl, sph);
+        if (++sl == kF8Ring) {
+          sl = 0;
+          sph ^= 1;
+        }
+      };
+      for (int64_t tile = pair; tile < ntiles; tile += npairs) {
+        factors(0);
         for (int kb = 0; kb < kblocks; ++kb) {
-          if ((kb & (kF8Group - 1)) == 0) {
-            if (!*abort_flag) wait(f_full, sl, sph);
-            if (++sl == kF8Ring) {
-              sl = 0;
-              sph ^= 1;
-            }
-          }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
+            if (h == 1 && kb + 1 < kblocks) factors(kb + 1);
             if (!*abort_flag) wait(t_full, 2 * buf + h, ph);
             __syncwarp();
-            asm volatile("bar.arrive %0, %1;" ::"r"(1 + 2 * buf + h), "n"(32 * (kF8EpiWarps + 1)) : "memory");
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+              asm volatile("bar.arrive %0, %1;" ::"r"(1 + kF8Acc * p + 2 * buf + h), "n"(32 * (kF8EpiWarps / 2 + 1)) : "memory");
           }
           ph ^= buf;
           buf ^= 1;
         }
+      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kF8EpiRegs));
     // ---- epilogue ------------------------------------------------------------------------------
     const int part = warp >> 2;
     const int warp_row = (warp & 3) * 32, row = warp_row + lane;
-    const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp_row) << 16) + part * 32;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp_row) << 16) ;
+    const int col0 = MODE == kFp8GateUp ? part * 32 : part * 64, col1 = MODE == kFp8GateUp ? 64 + part * 32 : part * 64 + 32;
     const uint32_t released = f8_of_rank(&t_empty[0], 0);
-    unsigned char* buf_out = out_buf + warp * kF8StoreBytes;
+    unsigned char* buf_out = out_buf + warp * f8_store_bytes<MODE>;
     int buf = 0, sl = 0, par = 0;
+    // The two column parts go by barriers of their own: warps w and w + 4 share a scheduler, and one
+    // adds while the other waits for its load.
     auto ready = [&](int ac) {
-      asm volatile("bar.sync %0, %1;" ::"r"(1 + ac), "n"(32 * (kF8EpiWarps + 1)) : "memory");
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + kF8Acc * part + ac), "n"(32 * (kF8EpiWarps / 2 + 1)) : "memory");
       tc_fence_after();
     };
     auto release = [&](int ac) {
@@ -461,7 +517,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
       const int pos0 = g.y + static_cast<int>(rank) * kF8Rows;
       const int rows = g.z - static_cast<int>(rank) * kF8Rows;  // of this CTA; may be <= 0
       const bool live = row < rows, warp_live = warp_row < rows;
-      float acc[2][2][32];  // [block][half][column]: column 64 half + 32 part + j of the block
+      float acc[2][2][32];  // [col0, col1][half of the k-block's accumulators][column]
 #pragma unroll
       for (int j = 0; j < 32; ++j) acc[0][0][j] = acc[0][1][j] = acc[1][0][j] = acc[1][1][j] = 0.f;
       if (warp_live) {
@@ -471,10 +527,15 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
         const float2* fr = ring + row;
         float2 f, fn = make_float2(0.f, 0.f);
         ready(2 * buf);
-        f = fr[sl * kF8Group * kF8Rows];
-        group_read(0);
-        f8_ld32(lane_base + 2 * buf * kF8AccCols, v0);
-        f8_ld32(lane_base + 2 * buf * kF8AccCols + 64, v1);
+        auto factors = [&](int kb) {
+          float2 t = fr[(sl * kF8Group + (kb & (kF8Group - 1))) * kF8Rows];
+          if (MODE != kFp8GateUp) t.x = t.y = part ? t.y : t.x;  // one weight block
+          group_read(kb);
+          return t;
+        };
+        f = factors(0);
+        f8_ld32(lane_base + 2 * buf * kF8AccCols + col0, v0);
+        f8_ld32(lane_base + 2 * buf * kF8AccCols + col1, v1);
         for (int kb = 0; kb < kblocks; ++kb) {
           const uint32_t d = lane_base + 2 * buf * kF8AccCols, dn = lane_base + 2 * (buf ^ 1) * kF8AccCols;
           f8_ld_wait(v0);
@@ -482,22 +543,21 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
           release(2 * buf);
           f8_accumulate(acc[0][0], v0, f.x);
           ready(2 * buf + 1);
-          f8_ld32(d + kF8AccCols, v0);
+          f8_ld32(d + kF8AccCols + col0, v0);
+          const bool more = kb + 1 < kblocks;
+          if (more) fn = factors(kb + 1);
           f8_accumulate(acc[1][0], v1, f.y);
-          f8_ld32(d + kF8AccCols + 64, v1);
+          f8_ld32(d + kF8AccCols + col1, v1);
           f8_ld_wait(v0);
           f8_ld_wait(v1);
           release(2 * buf + 1);
           f8_accumulate(acc[0][1], v0, f.x);
-          const bool more = kb + 1 < kblocks;
           if (more) {
             ready(2 * (buf ^ 1));
-            fn = fr[(sl * kF8Group + ((kb + 1) & (kF8Group - 1))) * kF8Rows];
-            group_read(kb + 1);
-            f8_ld32(dn, v0);
+            f8_ld32(dn + col0, v0);
           }
           f8_accumulate(acc[1][1], v1, f.y);
-          if (more) f8_ld32(dn + 64, v1);
+          if (more) f8_ld32(dn + col1, v1);
           f = fn;
           buf ^= 1;
         }
@@ -563,14 +623,10 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
             o = static_cast<int64_t>(slot / a.s) * a.out_stride + static_cast<int64_t>(slot % a.s) * a.out_stride_s;
           }
         }
-        const int c = 2 * ni * kFp8Block + part * 32;
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            f8_store32(a.out, o, acc[b][h], c + b * kFp8Block + h * 64, a.n, a.out_dtype, a.out_vec, buf_out);
+        f8_store_rows(a.out, o, acc, (2 * ni + part) * kFp8Block, a.n, a.out_dtype, a.out_vec, buf_out);
       }
     }
+    if (MODE != kFp8GateUp) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
   __syncthreads();
