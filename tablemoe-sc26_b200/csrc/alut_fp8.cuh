@@ -138,15 +138,21 @@ struct Fp8Route {
   int64_t sel_stride;
   const uint8_t* compute;  // NULL: every slot
   int64_t compute_stride;
+  int flat;                // sel and compute are contiguous
   uint32_t* err;
 };
 
 // The expert of slot i, or -1 if the slot is not computed (or names no expert).
 __device__ __forceinline__ int fp8_slot_expert(const Fp8Route& r, int i, bool& bad) {
-  const uint32_t q = static_cast<uint32_t>(i) / static_cast<uint32_t>(r.s);
-  const int64_t t = q, s = i - static_cast<int>(q) * r.s;
-  const int64_t e = r.sel[t * r.sel_stride + s];  // both loads at once
-  if (r.compute && !r.compute[t * r.compute_stride + s]) return -1;
+  int64_t at = i, cat = i;
+  if (!r.flat) {  // rows with gaps: the token's row and the slot in it
+    const uint32_t t = static_cast<uint32_t>(i) / static_cast<uint32_t>(r.s);
+    const int s = i - static_cast<int>(t) * r.s;
+    at = t * r.sel_stride + s;
+    cat = t * r.compute_stride + s;
+  }
+  const int64_t e = r.sel[at];  // both loads at once
+  if (r.compute && !r.compute[cat]) return -1;
   if (e < 0 || e >= r.e) {
     bad = true;
     return -1;
@@ -301,18 +307,17 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 2) k_fp8_stream(StreamArgs 
     cnt = 0;
 #pragma unroll
     for (int i = 0; i < kStreamMaxSlots / 32; ++i) {
+      if (32 * i >= n || cnt == kStreamRows) continue;
       unsigned hits = __ballot_sync(kAll, ids[i] == mine);
       if (32 * i <= y) {
         const unsigned below = y - 32 * i < 32 ? (1u << (y - 32 * i)) - 1u : kAll;
         before += __popc(hits & below);
         hits &= ~below;
       }
-      while (hits && cnt < kStreamRows) {
-        const int b = __ffs(hits) - 1;
-        hits &= hits - 1;
-        if (lane == cnt) member = 32 * i + b;
-        ++cnt;
-      }
+      // lane m takes the (m - cnt)-th of them
+      const unsigned mine_bit = __fns(hits, 0, lane - cnt + 1);
+      if (lane >= cnt && lane < kStreamRows && mine_bit < 32) member = 32 * i + mine_bit;
+      cnt = min(kStreamRows, cnt + __popc(hits));
     }
     if (before % kStreamRows) return;
   }
@@ -325,33 +330,38 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 2) k_fp8_stream(StreamArgs 
   const int64_t tile_stride = MODE == kFp8GateUp ? a.w_stride_half : kStreamWRows * a.w_stride;
   // Every row and column of the slice is there: no copy needs to look.
   const bool whole = (a.k & (kFp8Block - 1)) == 0 && r0 + steps * all <= a.n;
-  auto issue = [&](int step, int kb, int stage) {  // this warp's operands of one step
-    const uint8_t* p = wbase + static_cast<int64_t>(step) * all * a.w_stride + kb * kFp8Block;
-    uint4* dst = ring + stage * kStreamStepUnits;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint8_t* src = p + i * tile_stride + h * 8 * a.w_stride + 64 * j;
-          uint4* d = dst + (i * 4 + h * 2 + j) * 32;
-          if (whole) {
-            cp_async16(d, src);
-          } else {
-            const int row = row0 + step * all + (MODE == kFp8GateUp ? 0 : i * kStreamWRows) + 8 * h + g;
-            const int bytes = row < a.n ? max(0, min(16, a.k - (kb * kFp8Block + 16 * c + 64 * j))) : 0;
-            cp_async16_part(d, bytes > 0 ? src : a.w, bytes);
-          }
-        }
-  };
   int istep = 0, ij = 0;  // the next to issue: for each step's rows, this warp's k-blocks
+  const uint8_t* ip = wbase + ki * kFp8Block;
+  const int64_t high = 8 * a.w_stride, next_kb = static_cast<int64_t>(ks) * kFp8Block;
+  const int64_t next_step = static_cast<int64_t>(all) * a.w_stride - (mykb - 1) * next_kb;
   auto issue_next = [&](int stage) {
     if (istep < steps) {
-      issue(istep, ki + ij * ks, stage);
+      uint4* dst = ring + stage * kStreamStepUnits;
+      if (whole) {
+        const uint8_t* src = ip;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          cp_async16(dst + (i * 4) * 32, src);
+          cp_async16(dst + (i * 4 + 1) * 32, src + 64);
+          cp_async16(dst + (i * 4 + 2) * 32, src + high);
+          cp_async16(dst + (i * 4 + 3) * 32, src + high + 64);
+          src += tile_stride;
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int i = u >> 2, h = (u >> 1) & 1, j = u & 1;
+          const int row = row0 + istep * all + (MODE == kFp8GateUp ? 0 : i * kStreamWRows) + 8 * h + g;
+          const int bytes = row < a.n ? max(0, min(16, a.k - ((ki + ij * ks) * kFp8Block + 16 * c + 64 * j))) : 0;
+          cp_async16_part(dst + u * 32, bytes > 0 ? ip + i * tile_stride + h * high + 64 * j : a.w, bytes);
+        }
+      }
       if (++ij == mykb) {
         ij = 0;
         ++istep;
+        ip += next_step;
+      } else {
+        ip += next_kb;
       }
     }
     cp_async_commit();  // one group per step, empty behind the last

@@ -118,6 +118,7 @@ static int launch_tc(const CUtensorMap& xm, const CUtensorMap& wm, const F8Args&
   auto kern = k_fp8_tc<MODE>;
   const int rc = allow_smem(reinterpret_cast<const void*>(kern), f8_smem_bytes<MODE>);
   if (rc) return rc;
+  if (max_tiles + num_sms() > 0x7fffffffll) return fail(ALUT_ERANGE, "fp8: %lld tiles", static_cast<long long>(max_tiles));
   const unsigned grid = 2 * static_cast<unsigned>(std::min<int64_t>(max_tiles, num_sms() / 2));  // pairs of CTAs
   const cudaError_t e = launch_pdl(kern, dim3(grid), dim3(kF8Threads), f8_smem_bytes<MODE>, st, xm, wm, a);
   if (e != cudaSuccess) return fail(ALUT_ECUDA, "k_fp8_tc: %s", cudaGetErrorString(e));
@@ -125,9 +126,9 @@ static int launch_tc(const CUtensorMap& xm, const CUtensorMap& wm, const F8Args&
 }
 
 static int launch_rows(const F8PrepArgs& a, int x_dtype, cudaStream_t st) {
-  const int64_t n = static_cast<int64_t>(a.rows) * fp8_blocks(a.k);
-  const unsigned grid = static_cast<unsigned>(
-      std::max<int64_t>(1, std::min<int64_t>((n + 15) / 16, std::max<int64_t>((n + 63) / 64, 4 * num_sms()))));
+  const int64_t units = static_cast<int64_t>(a.rows) * ceil_div(fp8_blocks(a.k), kF8RowBlocks);
+  if (units + 8 > 0x7fffffffll) return fail(ALUT_ERANGE, "fp8: %d rows of %d columns", a.rows, a.k);
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((units + 7) / 8, kF8RowCtas * num_sms()));
   auto kern = x_dtype == ALUT_BF16 ? k_fp8_rows<__nv_bfloat16> : x_dtype == ALUT_F16 ? k_fp8_rows<__half> : k_fp8_rows<float>;
   if (!a.place) {
     kern<<<grid, 256, 0, st>>>(a);
@@ -326,7 +327,8 @@ int alut_experts_fp8(const alut_fp8_experts_t* ex, int32_t q, int32_t s, const v
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   char* base = static_cast<char*>(workspace);
   const int n = q * s;
-  Fp8Route r{q, s, ex->num_experts, sel, sel_stride, compute, compute_stride, error_bits};
+  Fp8Route r{q, s, ex->num_experts, sel, sel_stride, compute, compute_stride,
+             sel_stride == s && (!compute || compute_stride == s), error_bits};
   if (!experts_stream(ex, n)) {
     F8PrepArgs p{};
     p.x = x;

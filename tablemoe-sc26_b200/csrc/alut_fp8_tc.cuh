@@ -26,9 +26,9 @@
 //   barriers:  full/empty per stage, full/empty per accumulator, full/empty per ring slot; the
 //              stages' full and the accumulators' empty count in the leader, the commits arrive in
 //              both CTAs
-// Linear and Down end with a row segment of 128 outputs per thread, written to shared memory and from
-// there by one bulk copy per row, which runs on while the next tile is added up (with store
-// instructions a tile's end took 4000 cycles: a fifth of the whole product of 8192 x 4096 outputs).
+// Linear and Down end with a row segment of 128 outputs per thread, which goes out through shared
+// memory so that a store instruction writes 256 adjacent bytes of two rows (one bulk copy per row
+// instead took 2400 cycles a warp to issue).
 // GateUp ends with h = silu(gate) * up, its 8-bit form (the 128 hidden units of the tile are one
 // block of the next product; the two column halves exchange their maxima) written for Down.
 // x's rows lie in the order of the plan (k_fp8_rows writes a token's 8-bit row once per computed
@@ -57,9 +57,9 @@ constexpr uint32_t kF8TileBytes = kF8Rows * kFp8Block;  // one 128 x 128 operand
 constexpr uint32_t kF8StageBytes = 2 * kF8TileBytes;    // x's rows, a weight block
 constexpr int kF8EpiWarps = 8;
 // Three warpgroups, launched with 168 registers a thread; the epilogue's two need more (128 sums, 64
-// loaded values), the third fewer: 2 x 232 + 40 = 3 x 168.
+// loaded values), the third fewer: 2 x 224 + 56 = 3 x 168.
 constexpr int kF8Threads = 32 * (kF8EpiWarps + 4);
-constexpr int kF8EpiRegs = 232, kF8RoleRegs = 40;
+constexpr int kF8EpiRegs = 224, kF8RoleRegs = 56;
 constexpr int kF8CopyWarp = kF8EpiWarps, kF8MmaWarp = kF8EpiWarps + 1, kF8ScaleWarp = kF8EpiWarps + 2, kF8WaitWarp = kF8EpiWarps + 3;
 constexpr int kF8Group = 4, kF8Ring = 2;     // factors of 4 k-blocks per ring slot
 constexpr uint32_t kF8RowBytes = 256 + 16;    // an output row on its way out (padded: no bank conflicts)
@@ -110,6 +110,15 @@ __device__ __forceinline__ bool f8_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool f8_test(uint32_t bar, uint32_t parity) {  // a look, without waiting
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
       : "=r"(ok)
       : "r"(bar), "r"(parity)
       : "memory");
@@ -237,10 +246,7 @@ __device__ __forceinline__ uint32_t f8_unit(int r, int c) {
 }
 
 // Output rows. A thread has 64 or 128 columns (from c0 on) of its row (offset o; negative: no row):
-// into its own padded row of the warp's buffer, then one bulk copy of the row segment.
-__device__ __forceinline__ void f8_rows_reusable() {  // this thread's copies have read their rows
-  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-}
+// into its own padded row of the warp's buffer, the offset behind it; then two rows at a time out.
 template <typename TO, int C>
 __device__ __forceinline__ void f8_store_row(TO* out, int64_t o, const float (&v)[C], int c0, int n, bool vec,
                                              unsigned char* rows) {
@@ -248,7 +254,7 @@ __device__ __forceinline__ void f8_store_row(TO* out, int64_t o, const float (&v
   constexpr int kPer = 16 / sizeof(TO);
   const int lane = threadIdx.x & 31;
   unsigned char* mine = rows + lane * kF8RowBytes;
-  f8_rows_reusable();
+  __syncwarp();
 #pragma unroll
   for (int c = 0; c < C; c += kPer) {
     __align__(16) TO t[kPer];
@@ -256,23 +262,28 @@ __device__ __forceinline__ void f8_store_row(TO* out, int64_t o, const float (&v
     for (int j = 0; j < kPer; ++j) t[j] = from_f32<TO>(v[c + j]);
     *reinterpret_cast<uint4*>(mine + c * sizeof(TO)) = *reinterpret_cast<const uint4*>(t);
   }
+  *reinterpret_cast<int64_t*>(mine + 256) = o;
+  __syncwarp();
   const int have = min(C, n - c0);  // may be <= 0
   if (vec && have % kPer == 0) {
-    fence_async_shared();
-    if (o >= 0 && have > 0)
-      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(out + o + c0), "r"(smem_addr(mine)),
-                   "r"(have * static_cast<int>(sizeof(TO)))
-                   : "memory");
-    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    const int c = (lane & 15) * kPer;
+    const unsigned char* from = rows + (lane >> 4) * kF8RowBytes;
+    TO* to = out + c0 + c;
+    if (c < have) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int64_t ro = *reinterpret_cast<const int64_t*>(from + 2 * i * kF8RowBytes + 256);
+        const uint4 u = *reinterpret_cast<const uint4*>(from + 2 * i * kF8RowBytes + (lane & 15) * 16);
+        if (ro >= 0) *reinterpret_cast<uint4*>(to + ro) = u;
+      }
+    }
   } else {  // a ragged edge, or rows that do not start on 16 bytes: element by element along the rows
-    __syncwarp();
     for (int r = 0; r < 32; ++r) {
-      const int64_t ro = __shfl_sync(0xffffffffu, o, r);
+      const int64_t ro = *reinterpret_cast<const int64_t*>(rows + r * kF8RowBytes + 256);
       if (ro < 0) continue;
       for (int c = lane; c < have; c += 32)
         out[ro + c0 + c] = *reinterpret_cast<const TO*>(rows + r * kF8RowBytes + c * sizeof(TO));
     }
-    __syncwarp();
   }
 }
 // acc[i][h][j]: column c0 + 64 h + 32 i + j.
@@ -351,9 +362,26 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
   pdl_wait();  // the 8-bit rows, the plan and the scales come from the kernel before
   const int nt = MODE == kFp8GateUp ? nblocks : (nblocks + 1) / 2;  // tiles along the weight rows
   const int mt = MODE == kFp8Linear ? (a.m + kF8PairRows - 1) / kF8PairRows : __ldcg(a.n_groups);
-  const int64_t ntiles = static_cast<int64_t>(mt) * nt;
+  const int ntiles = mt * nt;  // (the host refuses more than fit)
+  const int step_m = npairs / nt, step_n = npairs % nt;
+  // The tiles of this pair, without a division per tile: row tile mi, column tile ni.
+  struct Tile {
+    int i, mi, ni;
+  };
+  auto first_tile = [&]() { return Tile{pair, pair / nt, pair % nt}; };
+  auto next_tile = [&](Tile t) {
+    t.i += npairs;
+    t.mi += step_m;
+    t.ni += step_n;
+    if (t.ni >= nt) {
+      t.ni -= nt;
+      ++t.mi;
+    }
+    return t;
+  };
   // A pair tile: expert, first row (position) and number of rows.
   auto tile_rows = [&](int mi) {
+    if (mi >= mt) return make_int4(0, 0, 0, 0);
     if constexpr (MODE == kFp8Linear) return make_int4(0, mi * kF8PairRows, min(kF8PairRows, a.m - mi * kF8PairRows), 0);
     else return __ldcg(a.groups + mi);
   };
@@ -369,9 +397,13 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
     if (warp == kF8CopyWarp) {
       // ---- TMA copies --------------------------------------------------------------------------
       int st = 0, past = 1;
-      for (int64_t tile = pair; tile < ntiles && !stopped(); tile += npairs) {
-        const int mi = static_cast<int>(tile / nt), ni = static_cast<int>(tile % nt);
-        const int4 g = tile_rows(mi);
+      Tile next = first_tile();  // every role reads its next tile's rows a tile ahead
+      int4 ahead = tile_rows(next.mi);
+      while (next.i < ntiles && !stopped()) {
+        const int ni = next.ni;
+        const int4 g = ahead;
+        next = next_tile(next);
+        ahead = tile_rows(next.mi);
         const bool second = g.z > kF8Rows;  // the second CTA has rows
         const uint32_t bytes = kF8TileBytes * (second ? 4 : 3);
         const int wrow = MODE == kFp8GateUp ? ni * kFp8Block : (2 * ni + static_cast<int>(rank)) * kFp8Block;
@@ -393,37 +425,46 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
       // ---- MMA issuer ----------------------------------------------------------------------------
       if (rank == 0) {
         int st = 0, ph = 0, buf = 0, past = 1;
-        const uint32_t done0 = smem_addr(t_full), freed0 = smem_addr(empty);
+        const uint32_t done0 = smem_addr(t_full), freed0 = smem_addr(empty), full0 = smem_addr(full), empty0 = smem_addr(t_empty);
+        bool seen_full = false, seen0 = false, seen1 = false;
         const uint32_t idesc = f8_idesc();
         const uint64_t desc0 = pt_desc_sw128(smem_addr(stages));  // + address / 16 within the first 14 bits
-        for (int64_t tile = pair; tile < ntiles && !stopped(); tile += npairs) {
+        for (int tile = pair; tile < ntiles && !stopped(); tile += npairs) {
           for (int kb = 0; kb < kblocks; ++kb) {
-            wait(full, st, ph);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {  // accumulator 2 buf + h, used once per two k-blocks
-              const int acc = 2 * buf + h;
-              wait(t_empty, acc, past);
-              tc_fence_after();
-              const uint64_t dx = desc0 + static_cast<uint32_t>(st) * (kF8StageBytes >> 4);
-              const uint64_t dw = dx + ((kF8TileBytes + h * kF8TileBytes / 2) >> 4);
-              if (h) f8_issue<true>(tmem + acc * kF8AccCols, dx, dw, idesc, done0 + 8 * acc, freed0 + 8 * st);
-              else f8_issue<false>(tmem + acc * kF8AccCols, dx, dw, idesc, done0 + 8 * acc, 0);
-            }
+            // accumulators 2 buf and 2 buf + 1, each used once per two k-blocks
+            const uint64_t dx = desc0 + static_cast<uint32_t>(st) * (kF8StageBytes >> 4), dw = dx + (kF8TileBytes >> 4);
+            const uint32_t d = tmem + 2 * buf * kF8AccCols, done = done0 + 16 * buf, freed = freed0 + 8 * st;
+            if (!seen_full) wait(full, st, ph);
+            if (!seen0) wait(t_empty, 2 * buf, past);
+            tc_fence_after();
+            f8_issue<false>(d, dx, dw, idesc, done, 0);
+            if (!seen1) wait(t_empty, 2 * buf + 1, past);
+            tc_fence_after();
             if (++st == kStages) {
               st = 0;
               ph ^= 1;
             }
             past ^= buf;
             buf ^= 1;
+            // A look at the next k-block's barriers: the answers arrive behind this issue. (A wait
+            // costs 100 cycles and more even where it is over, three of them more than the MMAs.)
+            seen_full = f8_test(full0 + 8 * st, ph);
+            seen0 = f8_test(empty0 + 16 * buf, past);
+            seen1 = f8_test(empty0 + 16 * buf + 8, past);
+            f8_issue<true>(d + kF8AccCols, dx, dw + (kF8TileBytes >> 5), idesc, done + 8, freed);
           }
         }
       }
     } else if (warp == kF8ScaleWarp) {
       // ---- factors -----------------------------------------------------------------------------
+      // A ring slot's 24 values are loaded together, and the next slot's before this one's are
+      // written: loads one k-block at a time made this warp the bottleneck (their L2 latency, 860
+      // cycles a k-block).
       int sl = 0, past = 1;
-      for (int64_t tile = pair; tile < ntiles && !stopped(); tile += npairs) {
-        const int mi = static_cast<int>(tile / nt), ni = static_cast<int>(tile % nt);
-        const int4 g = tile_rows(mi);
+      Tile next = first_tile();
+      int4 g = tile_rows(next.mi);
+      while (next.i < ntiles && !stopped()) {
+        const int ni = next.ni;
         const int rows = min(kF8Rows, g.z - static_cast<int>(rank) * kF8Rows);  // may be <= 0
         const float* sx = a.sx + g.y + rank * kF8Rows + lane;
         const int nb0 = MODE == kFp8GateUp ? ni : 2 * ni;
@@ -431,24 +472,34 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
         // the second block: the up rows' scales, or the next block of columns (none past the last)
         const float* sw1 = MODE == kFp8GateUp ? sw0 + static_cast<int64_t>(nblocks) * kblocks
                                               : (nb0 + 1 < nblocks ? sw0 + kblocks : sw0);
-        for (int kb = 0; kb < kblocks; ++kb) {
-          float s[4];
+        next = next_tile(next);
+        g = tile_rows(next.mi);  // (ahead of its use)
+        float s[kF8Group][4], w[kF8Group][2];
+        auto load = [&](int kb0) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[j] = lane + 32 * j < rows ? __ldcg(sx + 32 * j) : 0.f;
-          const float w0 = __ldg(sw0 + kb), w1 = __ldg(sw1 + kb);
-          sx += a.scale_rows;
-          const int in = kb & (kF8Group - 1);
-          if (in == 0) wait(f_empty, sl, past);
+          for (int i = 0; i < kF8Group; ++i) {
+            const bool on = kb0 + i < kblocks;
+            const float* p = sx + (kb0 + i) * a.scale_rows;
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            ring[(sl * kF8Group + in) * kF8Rows + lane + 32 * j] = make_float2(s[j] * w0, s[j] * w1);
-          if (in == kF8Group - 1 || kb == kblocks - 1) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&f_full[sl]);
-            if (++sl == kF8Ring) {
-              sl = 0;
-              past ^= 1;
-            }
+            for (int j = 0; j < 4; ++j) s[i][j] = on && lane + 32 * j < rows ? __ldcg(p + 32 * j) : 0.f;
+            w[i][0] = on ? __ldg(sw0 + kb0 + i) : 0.f;
+            w[i][1] = on ? __ldg(sw1 + kb0 + i) : 0.f;
+          }
+        };
+        load(0);
+        for (int kb0 = 0; kb0 < kblocks; kb0 += kF8Group) {
+          wait(f_empty, sl, past);
+#pragma unroll
+          for (int i = 0; i < kF8Group; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              ring[(sl * kF8Group + i) * kF8Rows + lane + 32 * j] = make_float2(s[i][j] * w[i][0], s[i][j] * w[i][1]);
+          if (kb0 + kF8Group < kblocks) load(kb0 + kF8Group);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&f_full[sl]);
+          if (++sl == kF8Ring) {
+            sl = 0;
+            past ^= 1;
           }
         }
       }
@@ -466,7 +517,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
           sph ^= 1;
         }
       };
-      for (int64_t tile = pair; tile < ntiles; tile += npairs) {
+      for (int tile = pair; tile < ntiles; tile += npairs) {
         factors(0);
         for (int kb = 0; kb < kblocks; ++kb) {
 #pragma unroll
@@ -511,12 +562,23 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
         if (++sl == kF8Ring) sl = 0;
       }
     };
-    for (int64_t tile = pair; tile < ntiles; tile += npairs, par ^= 1) {
-      const int mi = static_cast<int>(tile / nt), ni = static_cast<int>(tile % nt);
-      const int4 g = tile_rows(mi);
+    Tile next = first_tile();
+    int4 ahead = tile_rows(next.mi);
+    for (; next.i < ntiles; par ^= 1) {
+      const int ni = next.ni;
+      const int4 g = ahead;
+      next = next_tile(next);
+      ahead = tile_rows(next.mi);
       const int pos0 = g.y + static_cast<int>(rank) * kF8Rows;
       const int rows = g.z - static_cast<int>(rank) * kF8Rows;  // of this CTA; may be <= 0
       const bool live = row < rows, warp_live = warp_row < rows;
+      int64_t o = -1;  // where this thread's row of outputs begins
+      if (MODE == kFp8Linear && live) o = static_cast<int64_t>(pos0 + row) * a.out_stride;
+      if (MODE == kFp8Down && live) {
+        const int slot = __ldcg(a.sorted + pos0 + row);
+        const int t = slot / a.s;
+        o = t * a.out_stride + (slot - t * a.s) * a.out_stride_s;
+      }
       float acc[2][2][32];  // [col0, col1][half of the k-block's accumulators][column]
 #pragma unroll
       for (int j = 0; j < 32; ++j) acc[0][0][j] = acc[0][1][j] = acc[1][0][j] = acc[1][1][j] = 0.f;
@@ -573,13 +635,15 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
       }
       if constexpr (MODE == kFp8GateUp) {
         uint32_t m = 0;
+        if (warp_live) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {  // columns past I have zero weights: h = 0
-            acc[0][h][j] = silu_mul(acc[0][h][j], acc[1][h][j]);
-            m = max(m, abs_bits(acc[0][h][j]));
-          }
+            for (int j = 0; j < 32; ++j) {  // columns past I have zero weights: h = 0
+              acc[0][h][j] = silu_mul(acc[0][h][j], acc[1][h][j]);
+              m = max(m, abs_bits(acc[0][h][j]));
+            }
+        }
         s_max[par][part][row] = __uint_as_float(m);
         __syncwarp();
         if (lane == 0) mbar_arrive(maxima);
@@ -614,19 +678,9 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
         }
         if (live && part == 0) a.hs[ni * a.scale_rows + pos0 + row] = am / kE4m3Max;
       } else if (warp_live) {
-        int64_t o = -1;
-        if (live) {
-          if constexpr (MODE == kFp8Linear) {
-            o = static_cast<int64_t>(pos0 + row) * a.out_stride;
-          } else {
-            const int slot = __ldcg(a.sorted + pos0 + row);
-            o = static_cast<int64_t>(slot / a.s) * a.out_stride + static_cast<int64_t>(slot % a.s) * a.out_stride_s;
-          }
-        }
         f8_store_rows(a.out, o, acc, (2 * ni + part) * kFp8Block, a.n, a.out_dtype, a.out_vec, buf_out);
       }
     }
-    if (MODE != kFp8GateUp) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
   __syncthreads();
@@ -657,69 +711,109 @@ struct F8PrepArgs {
   int64_t out_stride, out_stride_s;
 };
 
-// x's 8-bit form: 16 lanes a block of 128 columns, 8 columns a lane, kF8RowUnroll blocks at a time.
-constexpr int kF8RowUnroll = 4;
+// x's 8-bit form. A warp takes kF8RowBlocks blocks of a row at a time, two side by side (16 lanes of 8
+// columns each); the next unit's loads are under way while this one is converted and stored. With
+// `place` the first unit overlaps the plan up to its stores.
+constexpr int kF8RowBlocks = 8;
+constexpr int kF8RowCtas = 4;  // per SM: 32 warps with 2 KB each on the way
 template <typename TX>
-__global__ void __launch_bounds__(256) k_fp8_rows(F8PrepArgs a) {
+struct F8Raw8 {  // 8 elements as they lie
+  uint4 w[sizeof(TX) / 2];
+};
+template <typename TX>
+__device__ __forceinline__ void f8_widen(const F8Raw8<TX>& r, float (&v)[8]) {
+  const TX* e = reinterpret_cast<const TX*>(&r);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = to_f32<TX>(e[j]);
+}
+template <typename TX>
+__global__ void __launch_bounds__(256, kF8RowCtas) k_fp8_rows(F8PrepArgs a) {
+  constexpr int kU = kF8RowBlocks / 2;
   pdl_launch_dependents();
-  const int kb = fp8_blocks(a.k);
-  const int64_t n = static_cast<int64_t>(a.rows) * kb;
-  const int sub = threadIdx.x & 15;
-  const int64_t step = (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 4;
-  if (a.place) pdl_wait();  // the plan
-  // whole warps iterate together (shuffles)
-  for (int64_t i0 = (static_cast<int64_t>(blockIdx.x) * blockDim.x + (threadIdx.x & ~31)) >> 4; i0 < n;
-       i0 += step * kF8RowUnroll) {
-    float v[kF8RowUnroll][8];
-    int row[kF8RowUnroll], b[kF8RowUnroll];
+  const int kb = fp8_blocks(a.k), chunks = (kb + kF8RowBlocks - 1) / kF8RowBlocks;
+  const int units = a.rows * chunks;  // (the host keeps them below 2^31)
+  const int step = gridDim.x * 8, step_r = step / chunks, step_c = step - step_r * chunks;
+  int unit = blockIdx.x * 8 + (threadIdx.x >> 5);
+  int row = unit / chunks, chunk = unit - row * chunks;
+  const int lane = threadIdx.x & 31, sub = lane & 15, side = lane >> 4;
+  auto fetch = [&](F8Raw8<TX> (&r)[kU], int row, int chunk) {
+    const TX* src = static_cast<const TX*>(a.x) + row * a.x_stride;
 #pragma unroll
-    for (int u = 0; u < kF8RowUnroll; ++u) {
-      const int64_t i = i0 + u * step + ((threadIdx.x >> 4) & 1);
-      row[u] = i < n ? static_cast<int>(i / kb) : -1;
-      b[u] = i < n ? static_cast<int>(i - static_cast<int64_t>(row[u]) * kb) : 0;
-      const int c = b[u] * kFp8Block + sub * 8;
-      const TX* src = static_cast<const TX*>(a.x) + static_cast<int64_t>(max(row[u], 0)) * a.x_stride;
-      if (row[u] >= 0 && a.x_vec && c + 8 <= a.k) {
-        load8<TX>(src + c, v[u]);
+    for (int u = 0; u < kU; ++u) {
+      const int c = (chunk * kF8RowBlocks + side + 2 * u) * kFp8Block + sub * 8;
+      if (a.x_vec && c + 8 <= a.k) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(TX) / 2); ++i) r[u].w[i] = __ldg(reinterpret_cast<const uint4*>(src + c) + i);
       } else {
+        TX* e = reinterpret_cast<TX*>(&r[u]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[u][j] = row[u] >= 0 && c + j < a.k ? to_f32<TX>(src[c + j]) : 0.f;
+        for (int j = 0; j < 8; ++j) e[j] = c + j < a.k ? src[c + j] : from_f32<TX>(0.f);
       }
     }
+  };
+  F8Raw8<TX> raw[kU];
+  if (unit < units) fetch(raw, row, chunk);
+  bool planned = !a.place;
+  while (unit < units) {
+    const int r = row, b0 = chunk * kF8RowBlocks + side;
+    uint2 q[kU];
+    float s[kU];
 #pragma unroll
-    for (int u = 0; u < kF8RowUnroll; ++u) {
+    for (int u = 0; u < kU; ++u) {
+      float v[8];
+      f8_widen<TX>(raw[u], v);
       uint32_t m = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[u][j]));
+      for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j]));
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      if (row[u] < 0) continue;
       const float am = fp8_amax(m);
-      const float f = kE4m3Max / am, s = am / kE4m3Max;
-      uint2 q;
-      q.x = e4m3x4(v[u][0] * f, v[u][1] * f, v[u][2] * f, v[u][3] * f);
-      q.y = e4m3x4(v[u][4] * f, v[u][5] * f, v[u][6] * f, v[u][7] * f);
-      const int c = b[u] * kFp8Block + sub * 8;
-      if (!a.place) {
-        *reinterpret_cast<uint2*>(a.xq + row[u] * f8_row_pitch(a.k) + c) = q;
-        if (sub == 0) a.sx[b[u] * a.scale_rows + row[u]] = s;
-        continue;
+      const float f = kE4m3Max / am;
+      s[u] = am / kE4m3Max;
+      q[u].x = e4m3x4(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
+      q[u].y = e4m3x4(v[4] * f, v[5] * f, v[6] * f, v[7] * f);
+    }
+    unit += step;
+    row += step_r;
+    chunk += step_c;
+    if (chunk >= chunks) {
+      chunk -= chunks;
+      ++row;
+    }
+    if (unit < units) fetch(raw, row, chunk);
+    auto put = [&](int64_t p) {
+      uint8_t* dst = a.xq + p * f8_row_pitch(a.k) + sub * 8;
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const int b = b0 + 2 * u;
+        if (b >= kb) break;
+        *reinterpret_cast<uint2*>(dst + b * kFp8Block) = q[u];
+        if (sub == 0) a.sx[b * a.scale_rows + p] = s[u];
       }
-      for (int t = 0; t < a.s; ++t) {
-        const int64_t p = a.place[static_cast<int64_t>(row[u]) * a.s + t];
-        if (p >= 0) {
-          *reinterpret_cast<uint2*>(a.xq + p * f8_row_pitch(a.k) + c) = q;
-          if (sub == 0) a.sx[b[u] * a.scale_rows + p] = s;
-        } else if (a.out) {
-          const int64_t o = row[u] * a.out_stride + t * a.out_stride_s + c;
+    };
+    if (!a.place) {
+      put(r);
+      continue;
+    }
+    if (!planned) pdl_wait();  // the plan
+    planned = true;
+    for (int t = 0; t < a.s; ++t) {
+      const int p = __ldcg(a.place + static_cast<int64_t>(r) * a.s + t);
+      if (p >= 0) {
+        put(p);
+      } else if (a.out) {
+        const int64_t o = r * a.out_stride + t * a.out_stride_s;
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          const int c = (b0 + 2 * u) * kFp8Block + sub * 8;
           if (a.out_vec && c + 8 <= a.k) {
             const float z[8] = {};
-            if (a.out_dtype == ALUT_BF16) store8(static_cast<__nv_bfloat16*>(a.out) + o, z);
-            else if (a.out_dtype == ALUT_F16) store8(static_cast<__half*>(a.out) + o, z);
-            else store8(static_cast<float*>(a.out) + o, z);
+            if (a.out_dtype == ALUT_BF16) store8(static_cast<__nv_bfloat16*>(a.out) + o + c, z);
+            else if (a.out_dtype == ALUT_F16) store8(static_cast<__half*>(a.out) + o + c, z);
+            else store8(static_cast<float*>(a.out) + o + c, z);
           } else {
             for (int j = 0; j < 8; ++j)
-              if (c + j < a.k) store_any(a.out, o + j, 0.f, a.out_dtype);
+              if (c + j < a.k) store_any(a.out, o + c + j, 0.f, a.out_dtype);
           }
         }
       }
