@@ -273,7 +273,9 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 2) k_fp8_stream(StreamArgs 
   uint4* xw = stream_smem + kStreamWarps * kStreamDepth * kStreamStepUnits;  // [kblocks][2][32]
   float* xs = reinterpret_cast<float*>(xw + kblocks * 64);              // [kblocks][8]
   float* sws = xs + kblocks * kStreamRows;                              // [steps][groups][2][kblocks]
-  pdl_launch_dependents();
+  // Only the down product may start early. What follows it may read its results without knowing that
+  // they are on their way (the lookups' combine), so the last kernel of a call lets nobody ahead.
+  if constexpr (MODE == kFp8GateUp) pdl_launch_dependents();
   // This CTA's rows: lane m < cnt holds the m-th (Linear: row, otherwise slot).
   int cnt, member = 0, expert = 0;
   if constexpr (MODE == kFp8Linear) {

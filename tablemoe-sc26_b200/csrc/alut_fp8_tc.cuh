@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
   const uint32_t rank = blockIdx.x & 1;  // in the pair
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
   const int kblocks = fp8_blocks(a.k), nblocks = fp8_blocks(a.n);
-  pdl_launch_dependents();
+  if constexpr (MODE == kFp8GateUp) pdl_launch_dependents();  // (a call's last kernel lets nobody ahead)
   if (warp == kF8MmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)),
                  "r"(kF8TmemCols)

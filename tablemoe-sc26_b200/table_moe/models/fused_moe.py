@@ -21,6 +21,7 @@ from __future__ import annotations
 import torch
 
 from ..cache_engine import VectorSearchEngine
+from ..ops.expert_routing import route_experts
 from ..ops.qwen_topk_softmax import route_for_lookup
 
 
@@ -30,7 +31,13 @@ class ALUTCachedMoE:
     ``run_experts(hidden_states, selected_experts, compute_mask, collected)`` must write the
     output of expert ``selected_experts[t, s]`` on token ``t`` into ``collected[t, s]`` for
     every slot with ``compute_mask[t, s]`` (the reference's expert loop writes
-    ``collected_expert_outputs`` the same way); other rows are ignored.
+    ``collected_expert_outputs`` the same way); other rows are ignored. A ``table_moe.ops.Fp8Experts``
+    is such a callable: the layer then runs without a host round trip or a Python loop.
+
+    ``router``: keyword arguments of ``table_moe.ops.route_experts`` (scoring, bias, n_group,
+    topk_group, group_rule, scale) for layers that do not route by a plain softmax.
+    ``shared``: a callable x -> [Q, H] whose result is added (shared experts, e.g.
+    ``Fp8SharedExpert``); called with ``out_dtype`` set to the value dtype.
 
     Defaults follow the Qwen3-VL wrapper: prefill keeps experts by importance
     (``KEEP_RATE``), decode keeps the first ``decode_keep_k`` slots; prefill searches with the
@@ -41,7 +48,7 @@ class ALUTCachedMoE:
 
     def __init__(self, manager, top_k, *, normalize_topk=False, prefill_keep="importance", prefill_keep_k=3,
                  decode_keep_k=3, keep_rate=0.6, prefill_variant="prefill_dot", decode_variant="decode_dot",
-                 renorm="to_one"):
+                 renorm="to_one", router=None, shared=None):
         self.engine = VectorSearchEngine(manager)
         self.manager = manager
         self.top_k = int(top_k)
@@ -50,14 +57,17 @@ class ALUTCachedMoE:
         self.decode_keep_k, self.keep_rate = decode_keep_k, keep_rate
         self.prefill_variant, self.decode_variant = prefill_variant, decode_variant
         self.renorm = renorm
+        self.router, self.shared = router, shared
 
     def route(self, router_logits, *, is_prefill, attn_scores=None):
         """(weights, selected_experts, compute_mask, reuse_mask) of ``_build_compute_mask``."""
         if is_prefill and self.prefill_keep == "importance":
-            return route_for_lookup(router_logits, self.top_k, normalize_topk=self.normalize_topk, keep="importance",
-                                    keep_rate=self.keep_rate, attn_scores=attn_scores)
-        k = self.prefill_keep_k if is_prefill else self.decode_keep_k
-        return route_for_lookup(router_logits, self.top_k, normalize_topk=self.normalize_topk, keep="fixed", keep_k=k)
+            keep = dict(keep="importance", keep_rate=self.keep_rate, attn_scores=attn_scores)
+        else:
+            keep = dict(keep="fixed", keep_k=self.prefill_keep_k if is_prefill else self.decode_keep_k)
+        if self.router is None:
+            return route_for_lookup(router_logits, self.top_k, normalize_topk=self.normalize_topk, **keep)
+        return route_experts(router_logits, self.top_k, normalize_topk=self.normalize_topk, **self.router, **keep)
 
     def __call__(self, hidden_states, router_logits, is_vision, run_experts, *, is_prefill, attn_scores=None,
                  return_routing=False):
@@ -66,9 +76,10 @@ class ALUTCachedMoE:
         values = self.manager.values_buffer
         collected = torch.empty((x.shape[0], self.top_k, values.shape[-1]), dtype=values.dtype, device=x.device)
         run_experts(x, sel, comp, collected)
+        base = None if self.shared is None else self.shared(x, out_dtype=values.dtype)  # the lookups add to it
         out = self.engine.lookup_combine(x, sel, is_vision.reshape(-1), reuse, w, compute_mask=comp,
                                          variant=self.prefill_variant if is_prefill else self.decode_variant,
-                                         renorm=self.renorm, computed=collected, return_hits=return_routing)
+                                         renorm=self.renorm, computed=collected, return_hits=return_routing, out=base)
         if return_routing:
             out, hit, idx = out
             return out, dict(weights=w, selected_experts=sel, compute_mask=comp, reuse_mask=reuse, hit=hit, idx=idx)
