@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "alut_fp8.cuh"
+#include "alut_fp8_grouped.cuh"
 #include "alut_fp8_tc.cuh"
 #include "alut_host.cuh"
 
@@ -113,15 +114,25 @@ static int encode_weight(CUtensorMap* map, const void* p, int k, int rows, int h
   return encode_map(map, p, 4, dims, strides, kF8Rows);
 }
 
-template <int MODE>
 static int launch_tc(const CUtensorMap& xm, const CUtensorMap& wm, const F8Args& a, int64_t max_tiles, cudaStream_t st) {
-  auto kern = k_fp8_tc<MODE>;
-  const int rc = allow_smem(reinterpret_cast<const void*>(kern), f8_smem_bytes<MODE>);
+  const int rc = allow_smem(reinterpret_cast<const void*>(k_fp8_tc), kF8SmemBytes);
   if (rc) return rc;
   if (max_tiles + num_sms() > 0x7fffffffll) return fail(ALUT_ERANGE, "fp8: %lld tiles", static_cast<long long>(max_tiles));
   const unsigned grid = 2 * static_cast<unsigned>(std::min<int64_t>(max_tiles, num_sms() / 2));  // pairs of CTAs
-  const cudaError_t e = launch_pdl(kern, dim3(grid), dim3(kF8Threads), f8_smem_bytes<MODE>, st, xm, wm, a);
+  const cudaError_t e = launch_pdl(k_fp8_tc, dim3(grid), dim3(kF8Threads), kF8SmemBytes, st, xm, wm, a);
   if (e != cudaSuccess) return fail(ALUT_ECUDA, "k_fp8_tc: %s", cudaGetErrorString(e));
+  return ALUT_OK;
+}
+
+template <int MODE>
+static int launch_grouped(const CUtensorMap& xm, const CUtensorMap& wm, const F8Args& a, int64_t max_tiles, cudaStream_t st) {
+  auto kern = k_fp8_grouped<MODE>;
+  const int rc = allow_smem(reinterpret_cast<const void*>(kern), kG8SmemBytes);
+  if (rc) return rc;
+  if (max_tiles + num_sms() > 0x7fffffffll) return fail(ALUT_ERANGE, "fp8: %lld tiles", static_cast<long long>(max_tiles));
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(max_tiles, num_sms()));
+  const cudaError_t e = launch_pdl(kern, dim3(grid), dim3(kF8Threads), kG8SmemBytes, st, xm, wm, a);
+  if (e != cudaSuccess) return fail(ALUT_ECUDA, "k_fp8_grouped: %s", cudaGetErrorString(e));
   return ALUT_OK;
 }
 
@@ -171,7 +182,7 @@ static ExpertsWorkspace experts_layout(const alut_fp8_experts_t* ex, int q, int 
   if (experts_stream(ex, n)) {
     w.hidden = off; off = align256(off + sizeof(float) * n * round_up(ex->i, 4));
   } else {
-    w.max_groups = ceil_div(n, kF8PairRows) + std::min<int64_t>(n, ex->num_experts);
+    w.max_groups = ceil_div(n, kG8Tokens) + std::min<int64_t>(n, ex->num_experts);
     w.n_groups = off; off = align256(off + sizeof(int));
     w.groups = off;   off = align256(off + sizeof(int4) * w.max_groups);
     w.sorted = off;   off = align256(off + sizeof(int) * n);
@@ -265,7 +276,10 @@ int alut_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, int32_t x_dt
     p.scale_rows = m;
     CUtensorMap xm, wm;
     rc = encode_rows(&xm, p.xq, m, k, kF8Rows);
-    if (!rc) rc = encode_weight(&wm, w, k, n, 1, 1, w_stride, 0, 0);
+    if (!rc) {
+      const uint64_t dims[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(n)}, strides[1] = {static_cast<uint64_t>(w_stride)};
+      rc = encode_map(&wm, w, 2, dims, strides, kF8Rows);
+    }
     if (!rc) rc = launch_rows(p, x_dtype, st);
     if (rc) return rc;
     F8Args a{};
@@ -280,7 +294,7 @@ int alut_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, int32_t x_dt
     a.out_stride = out_stride;
     a.out_vec = rows_vec(out, out_stride, out_dtype);
     a.err = error_bits;
-    return launch_tc<kFp8Linear>(xm, wm, a, static_cast<int64_t>(ceil_div(m, kF8PairRows)) * ((fp8_blocks(n) + 1) / 2), st);
+    return launch_tc(xm, wm, a, static_cast<int64_t>(ceil_div(m, kF8PairRows)) * ((fp8_blocks(n) + 1) / 2), st);
   }
   StreamArgs a{};
   a.x = x;
@@ -348,8 +362,8 @@ int alut_experts_fp8(const alut_fp8_experts_t* ex, int32_t q, int32_t s, const v
     p.out_stride_s = out_stride_s;
     uint8_t* hq = reinterpret_cast<uint8_t*>(base + ws.hidden);
     CUtensorMap xm, gm, hm, dm;
-    rc = encode_rows(&xm, p.xq, n, ex->h, kF8Rows);
-    if (!rc) rc = encode_rows(&hm, hq, n, ex->i, kF8Rows);
+    rc = encode_rows(&xm, p.xq, n, ex->h, kG8Step);
+    if (!rc) rc = encode_rows(&hm, hq, n, ex->i, kG8Step);
     if (!rc)
       rc = encode_weight(&gm, ex->gate_up, ex->h, ex->i, 2, ex->num_experts, ex->gate_up_stride[2],
                          ex->gate_up_stride[1], ex->gate_up_stride[0]);
@@ -361,7 +375,7 @@ int alut_experts_fp8(const alut_fp8_experts_t* ex, int32_t q, int32_t s, const v
     a.groups = reinterpret_cast<int4*>(base + ws.groups);
     a.n_groups = reinterpret_cast<int*>(base + ws.n_groups);
     k_fp8_plan<<<kF8PlanCtas, kF8PlanThreads, 2 * sizeof(int) * ex->num_experts, st>>>(
-        r, kF8PairRows, reinterpret_cast<int*>(base + ws.sorted), reinterpret_cast<int*>(base + ws.place),
+        r, kG8Tokens, reinterpret_cast<int*>(base + ws.sorted), reinterpret_cast<int*>(base + ws.place),
         reinterpret_cast<int4*>(base + ws.groups), reinterpret_cast<int*>(base + ws.n_groups));
     rc = check_launch("k_fp8_plan");
     if (rc) return rc;
@@ -376,7 +390,7 @@ int alut_experts_fp8(const alut_fp8_experts_t* ex, int32_t q, int32_t s, const v
     a.ws = ex->gate_up_scale;
     a.hq = hq;
     a.hs = reinterpret_cast<float*>(base + ws.hs);
-    rc = launch_tc<kFp8GateUp>(xm, gm, a, ws.max_groups * fp8_blocks(ex->i), st);
+    rc = launch_grouped<kFp8GateUp>(xm, gm, a, ws.max_groups * fp8_blocks(ex->i), st);
     if (rc) return rc;
     a.n = ex->h;
     a.k = ex->i;
@@ -387,7 +401,7 @@ int alut_experts_fp8(const alut_fp8_experts_t* ex, int32_t q, int32_t s, const v
     a.out_stride = out_stride_t;
     a.out_stride_s = out_stride_s;
     a.out_vec = p.out_vec;
-    return launch_tc<kFp8Down>(hm, dm, a, ws.max_groups * ((fp8_blocks(ex->h) + 1) / 2), st);
+    return launch_grouped<kFp8Down>(hm, dm, a, ws.max_groups * ((fp8_blocks(ex->h) + 1) / 2), st);
   }
   StreamArgs a{};
   a.r = r;

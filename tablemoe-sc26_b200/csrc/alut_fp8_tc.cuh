@@ -1,10 +1,9 @@
 // The block-scaled e4m3 product for many rows: tcgen05 (kind::f8f6f4), persistent pairs of CTAs.
 //
 // Tile of a pair (cta_group::2, one MMA of M = 256, N = 256 over both SMs): 256 rows of x, 128 per
-// CTA, x two 128-row weight blocks: adjacent output columns (Linear, Down), or the gate and the up
-// rows of the same 128 hidden units (GateUp). Each CTA loads its own rows of x and one of the two
-// weight blocks: 32 KB per 128 columns of K and CTA. With one CTA per tile it is 48 KB, and the
-// copies out of L2 and the operands' way through shared memory (48 KB in, 48 KB out, 128 bytes a
+// CTA, x two 128-row weight blocks, adjacent output columns. Each CTA loads its own rows of x and one
+// of the two weight blocks: 32 KB per 128 columns of K and CTA. With one CTA per tile it is 48 KB, and
+// the copies out of L2 and the operands' way through shared memory (48 KB in, 48 KB out, 128 bytes a
 // cycle) set the rate: 1040 cycles a k-block measured against 512 of the tensor cores.
 // The scales change with every 128 columns of K, so an accumulator holds one k-block only: the MMAs
 // of a k-block (4 steps of K = 32) overwrite it, and the epilogue warps add it, times sx[row, block]
@@ -15,8 +14,7 @@
 // issue, and reading it back (128 KB per SM through the TMEM port) takes 540. With two accumulators
 // of a whole k-block that chain ran at 1000 cycles a k-block.
 //
-//   warps 0-7  epilogue: TMEM lane quarter warp % 4; part warp / 4 has half the columns: GateUp 32 of
-//              the gate's 64 and the same 32 of the up's, otherwise one of the two weight blocks
+//   warps 0-7  epilogue: TMEM lane quarter warp % 4; part warp / 4 has one of the two weight blocks
 //   warp 8     TMA copies (128-byte swizzle), signalled to the leader CTA's barrier
 //   warp 9     MMA issuer (of the pair's leader, rank 0)
 //   warp 10    the factors sx sw of a k-block's 128 rows and two blocks, into a ring in shared
@@ -26,14 +24,9 @@
 //   barriers:  full/empty per stage, full/empty per accumulator, full/empty per ring slot; the
 //              stages' full and the accumulators' empty count in the leader, the commits arrive in
 //              both CTAs
-// Linear and Down end with a row segment of 128 outputs per thread, which goes out through shared
-// memory so that a store instruction writes 256 adjacent bytes of two rows (one bulk copy per row
-// instead took 2400 cycles a warp to issue).
-// GateUp ends with h = silu(gate) * up, its 8-bit form (the 128 hidden units of the tile are one
-// block of the next product; the two column halves exchange their maxima) written for Down.
-// x's rows lie in the order of the plan (k_fp8_rows writes a token's 8-bit row once per computed
-// slot), so all three products load plain tiles: gathering the rows here was slower (tile::gather4
-// moves a 128-byte row every 13 ns, 1.7 us a k-block; 16-byte cp.async by two warps 1.5 us).
+// A thread ends with a row segment of 128 outputs, which goes out through shared memory so that a
+// store instruction writes 256 adjacent bytes of two rows (one bulk copy per row instead took 2400
+// cycles a warp to issue).
 // Every wait is bounded in time (error bit, stop, time for what is in flight, TMEM freed).
 #pragma once
 
@@ -49,10 +42,7 @@ namespace alut {
 
 constexpr int kF8Rows = 128;                // rows of x per CTA
 constexpr int kF8PairRows = 2 * kF8Rows;    // per pair of CTAs
-// Stages of copies: as many as the memory beside the output rows holds.
-template <int MODE>
-constexpr int f8_stages = MODE == 1 /* kFp8GateUp */ ? 6 : 4;
-constexpr int kF8MaxStages = 6;
+constexpr int kF8Stages = 4;                // of copies: as many as the memory beside the output rows holds
 constexpr uint32_t kF8TileBytes = kF8Rows * kFp8Block;  // one 128 x 128 operand tile
 constexpr uint32_t kF8StageBytes = 2 * kF8TileBytes;    // x's rows, a weight block
 constexpr int kF8EpiWarps = 8;
@@ -63,13 +53,11 @@ constexpr int kF8EpiRegs = 224, kF8RoleRegs = 56;
 constexpr int kF8CopyWarp = kF8EpiWarps, kF8MmaWarp = kF8EpiWarps + 1, kF8ScaleWarp = kF8EpiWarps + 2, kF8WaitWarp = kF8EpiWarps + 3;
 constexpr int kF8Group = 4, kF8Ring = 2;     // factors of 4 k-blocks per ring slot
 constexpr uint32_t kF8RowBytes = 256 + 16;    // an output row on its way out (padded: no bank conflicts)
-template <int MODE>  // a warp's 32 of them; GateUp: 32 x 64 bytes
-constexpr uint32_t f8_store_bytes = MODE == 1 ? 32 * 64 : 32 * kF8RowBytes;
+constexpr uint32_t kF8StoreBytes = 32 * kF8RowBytes;  // a warp's 32 of them
 constexpr uint32_t kF8TmemCols = 512;
 constexpr int kF8Acc = 4, kF8AccCols = 128;  // accumulators
-template <int MODE>
-constexpr size_t f8_smem_bytes = 1024 + 1024 + static_cast<size_t>(f8_stages<MODE>) * kF8StageBytes +
-                                 kF8EpiWarps * f8_store_bytes<MODE> + kF8Ring * kF8Group * kF8Rows * sizeof(float2);
+constexpr size_t kF8SmemBytes = 1024 + 1024 + static_cast<size_t>(kF8Stages) * kF8StageBytes +
+                                kF8EpiWarps * kF8StoreBytes + kF8Ring * kF8Group * kF8Rows * sizeof(float2);
 
 // Scales of x's rows (and of the hidden rows) are kept [block][row]: a k-block's are adjacent.
 __host__ __device__ inline int64_t f8_row_pitch(int k) { return static_cast<int64_t>(fp8_blocks(k)) * kFp8Block; }
@@ -79,7 +67,7 @@ struct F8Args {
   const float* sx;          // x's scales [blocks k][scale_rows]
   int64_t scale_rows;       // rows (positions) in all
   const float* ws;          // weight scales, contiguous [E][halves][blocks n][blocks k]
-  const int4* groups;       // GateUp, Down: (expert, first position, rows, 0)
+  const int4* groups;       // GateUp, Down (alut_fp8_grouped.cuh): (expert, first position, rows, 0)
   const int* n_groups;
   const int* sorted;        // position -> slot
   int s;                    // slots per token
@@ -149,20 +137,12 @@ __device__ __forceinline__ bool f8_elect() {
 __device__ __forceinline__ void f8_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// TMA copies into this CTA's shared memory whose bytes count on a barrier of either CTA of the pair.
-__device__ __forceinline__ void f8_load_rows(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+// TMA copy into this CTA's shared memory whose bytes count on a barrier of either CTA of the pair.
+__device__ __forceinline__ void f8_load(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
       "%3}], [%4];" ::"r"(smem_addr(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ void f8_load_weight(void* dst, const CUtensorMap* map, int x, int y, int half, int e,
-                                               uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
-      "%3, %4, %5}], [%6];" ::"r"(smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(half), "r"(e), "r"(bar)
       : "memory");
 }
 // kind::f8f6f4 instruction descriptor: fp32 D, e4m3 A and B, K-major, M = 256, N = 128.
@@ -240,11 +220,6 @@ __device__ __forceinline__ void f8_accumulate(float (&sum)[32], const uint32_t (
   for (int j = 0; j < 32; ++j) sum[j] = fmaf(__uint_as_float(r[j]), f, sum[j]);
 }
 
-// 16-byte unit c of row r in a warp's 32 x 64-byte buffer: rows and columns without bank conflicts.
-__device__ __forceinline__ uint32_t f8_unit(int r, int c) {
-  return static_cast<uint32_t>(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
-}
-
 // Output rows. A thread has 64 or 128 columns (from c0 on) of its row (offset o; negative: no row):
 // into its own padded row of the warp's buffer, the offset behind it; then two rows at a time out.
 template <typename TO, int C>
@@ -306,23 +281,19 @@ __device__ __forceinline__ void f8_store_rows(void* out, int64_t o, const float 
   }
 }
 
-template <int MODE>
 __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
     k_fp8_tc(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, F8Args a) {
-  constexpr int kStages = f8_stages<MODE>;
   extern __shared__ unsigned char f8_raw[];
   unsigned char* f8_smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(f8_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(f8_smem);  // [kStages] (the leader's counts for the pair)
-  uint64_t* empty = full + kF8MaxStages;                  // [kStages]
-  uint64_t* t_full = empty + kF8MaxStages;                  // [kF8Acc]
+  uint64_t* full = reinterpret_cast<uint64_t*>(f8_smem);  // [kF8Stages] (the leader's counts for the pair)
+  uint64_t* empty = full + kF8Stages;                  // [kF8Stages]
+  uint64_t* t_full = empty + kF8Stages;                   // [kF8Acc]
   uint64_t* t_empty = t_full + kF8Acc;                    // [kF8Acc] (the leader's counts for the pair)
-  uint64_t* maxima = t_empty + kF8Acc;                    // [1] both column parts' maxima are there
-  uint64_t* f_full = maxima + 1;                          // [kF8Ring]
+  uint64_t* f_full = t_empty + kF8Acc;                    // [kF8Ring]
   uint64_t* f_empty = f_full + kF8Ring;                   // [kF8Ring]
-  unsigned char* stages = f8_smem + 1024;                 // [kStages][x rows | weight block]
-  float2* ring = reinterpret_cast<float2*>(stages + kStages * static_cast<size_t>(kF8StageBytes));  // [kF8Ring][kF8Group][kF8Rows]
+  unsigned char* stages = f8_smem + 1024;                 // [kF8Stages][x rows | weight block]
+  float2* ring = reinterpret_cast<float2*>(stages + kF8Stages * static_cast<size_t>(kF8StageBytes));  // [kF8Ring][kF8Group][kF8Rows]
   unsigned char* out_buf = reinterpret_cast<unsigned char*>(ring + kF8Ring * kF8Group * kF8Rows);    // output rows of 8 warps
-  __shared__ float s_max[2][2][kF8Rows];                  // [tile parity][column half][row]
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   volatile int* abort_flag = &s_abort;
@@ -330,7 +301,6 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
   const uint32_t rank = blockIdx.x & 1;  // in the pair
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
   const int kblocks = fp8_blocks(a.k), nblocks = fp8_blocks(a.n);
-  if constexpr (MODE == kFp8GateUp) pdl_launch_dependents();  // (a call's last kernel lets nobody ahead)
   if (warp == kF8MmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)),
                  "r"(kF8TmemCols)
@@ -338,7 +308,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < kF8Stages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
@@ -346,7 +316,6 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
       mbar_init(&t_full[i], 1);
       mbar_init(&t_empty[i], 2 * kF8EpiWarps);
     }
-    mbar_init(maxima, kF8EpiWarps);
     for (int i = 0; i < kF8Ring; ++i) {
       mbar_init(&f_full[i], 1);
       mbar_init(&f_empty[i], kF8EpiWarps);
@@ -359,9 +328,8 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
   f8_cluster_sync();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  pdl_wait();  // the 8-bit rows, the plan and the scales come from the kernel before
-  const int nt = MODE == kFp8GateUp ? nblocks : (nblocks + 1) / 2;  // tiles along the weight rows
-  const int mt = MODE == kFp8Linear ? (a.m + kF8PairRows - 1) / kF8PairRows : __ldcg(a.n_groups);
+  pdl_wait();  // x's 8-bit rows and scales come from the kernel before; no later kernel is let ahead
+  const int nt = (nblocks + 1) / 2, mt = (a.m + kF8PairRows - 1) / kF8PairRows;
   const int ntiles = mt * nt;  // (the host refuses more than fit)
   const int step_m = npairs / nt, step_n = npairs % nt;
   // The tiles of this pair, without a division per tile: row tile mi, column tile ni.
@@ -379,13 +347,6 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
     }
     return t;
   };
-  // A pair tile: expert, first row (position) and number of rows.
-  auto tile_rows = [&](int mi) {
-    if (mi >= mt) return make_int4(0, 0, 0, 0);
-    if constexpr (MODE == kFp8Linear) return make_int4(0, mi * kF8PairRows, min(kF8PairRows, a.m - mi * kF8PairRows), 0);
-    else return __ldcg(a.groups + mi);
-  };
-
   auto wait = [&](uint64_t* bars, int i, uint32_t parity) {  // a fresh barrier counts as past parity 1
     f8_wait(smem_addr(bars) + 8 * i, parity, abort_flag, a.err);
   };
@@ -397,26 +358,19 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
     if (warp == kF8CopyWarp) {
       // ---- TMA copies --------------------------------------------------------------------------
       int st = 0, past = 1;
-      Tile next = first_tile();  // every role reads its next tile's rows a tile ahead
-      int4 ahead = tile_rows(next.mi);
-      while (next.i < ntiles && !stopped()) {
-        const int ni = next.ni;
-        const int4 g = ahead;
-        next = next_tile(next);
-        ahead = tile_rows(next.mi);
-        const bool second = g.z > kF8Rows;  // the second CTA has rows
+      for (Tile t = first_tile(); t.i < ntiles && !stopped(); t = next_tile(t)) {
+        const bool second = a.m - t.mi * kF8PairRows > kF8Rows;  // the second CTA has rows
         const uint32_t bytes = kF8TileBytes * (second ? 4 : 3);
-        const int wrow = MODE == kFp8GateUp ? ni * kFp8Block : (2 * ni + static_cast<int>(rank)) * kFp8Block;
-        const int half = MODE == kFp8GateUp ? static_cast<int>(rank) : 0;
-        const int xrow = g.y + static_cast<int>(rank) * kF8Rows;
-        for (int kb = 0; kb < kblocks; ++kb, (++st == kStages ? (st = 0, past ^= 1) : 0)) {
+        const int wrow = (2 * t.ni + static_cast<int>(rank)) * kFp8Block;
+        const int xrow = t.mi * kF8PairRows + static_cast<int>(rank) * kF8Rows;
+        for (int kb = 0; kb < kblocks; ++kb, (++st == kF8Stages ? (st = 0, past ^= 1) : 0)) {
           wait(empty, st, past);
           if (f8_elect()) {
             unsigned char* sx = stages + static_cast<size_t>(st) * kF8StageBytes;
             const uint32_t bar = f8_of_rank(&full[st], 0);
             if (rank == 0) mbar_expect_tx(&full[st], bytes);
-            f8_load_weight(sx + kF8TileBytes, &w_map, kb * kFp8Block, wrow, half, g.x, bar);
-            if (rank == 0 || second) f8_load_rows(sx, &x_map, kb * kFp8Block, xrow, bar);
+            f8_load(sx + kF8TileBytes, &w_map, kb * kFp8Block, wrow, bar);
+            if (rank == 0 || second) f8_load(sx, &x_map, kb * kFp8Block, xrow, bar);
           }
           __syncwarp();
         }
@@ -440,7 +394,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
             f8_issue<false>(d, dx, dw, idesc, done, 0);
             if (!seen1) wait(t_empty, 2 * buf + 1, past);
             tc_fence_after();
-            if (++st == kStages) {
+            if (++st == kF8Stages) {
               st = 0;
               ph ^= 1;
             }
@@ -461,19 +415,12 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
       // written: loads one k-block at a time made this warp the bottleneck (their L2 latency, 860
       // cycles a k-block).
       int sl = 0, past = 1;
-      Tile next = first_tile();
-      int4 g = tile_rows(next.mi);
-      while (next.i < ntiles && !stopped()) {
-        const int ni = next.ni;
-        const int rows = min(kF8Rows, g.z - static_cast<int>(rank) * kF8Rows);  // may be <= 0
-        const float* sx = a.sx + g.y + rank * kF8Rows + lane;
-        const int nb0 = MODE == kFp8GateUp ? ni : 2 * ni;
-        const float* sw0 = a.ws + (static_cast<int64_t>(g.x) * (MODE == kFp8GateUp ? 2 : 1) * nblocks + nb0) * kblocks;
-        // the second block: the up rows' scales, or the next block of columns (none past the last)
-        const float* sw1 = MODE == kFp8GateUp ? sw0 + static_cast<int64_t>(nblocks) * kblocks
-                                              : (nb0 + 1 < nblocks ? sw0 + kblocks : sw0);
-        next = next_tile(next);
-        g = tile_rows(next.mi);  // (ahead of its use)
+      for (Tile t = first_tile(); t.i < ntiles && !stopped(); t = next_tile(t)) {
+        const int row0 = t.mi * kF8PairRows + static_cast<int>(rank) * kF8Rows;
+        const int rows = min(kF8Rows, a.m - row0);  // may be <= 0
+        const float* sx = a.sx + row0 + lane;
+        const float* sw0 = a.ws + static_cast<int64_t>(2 * t.ni) * kblocks;
+        const float* sw1 = 2 * t.ni + 1 < nblocks ? sw0 + kblocks : sw0;  // (none past the last)
         float s[kF8Group][4], w[kF8Group][2];
         auto load = [&](int kb0) {
 #pragma unroll
@@ -539,11 +486,11 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
     // ---- epilogue ------------------------------------------------------------------------------
     const int part = warp >> 2;
     const int warp_row = (warp & 3) * 32, row = warp_row + lane;
-    const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp_row) << 16) ;
-    const int col0 = MODE == kFp8GateUp ? part * 32 : part * 64, col1 = MODE == kFp8GateUp ? 64 + part * 32 : part * 64 + 32;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp_row) << 16);
+    const int col0 = part * 64, col1 = col0 + 32;
     const uint32_t released = f8_of_rank(&t_empty[0], 0);
-    unsigned char* buf_out = out_buf + warp * f8_store_bytes<MODE>;
-    int buf = 0, sl = 0, par = 0;
+    unsigned char* buf_out = out_buf + warp * kF8StoreBytes;
+    int buf = 0, sl = 0;
     // The two column parts go by barriers of their own: warps w and w + 4 share a scheduler, and one
     // adds while the other waits for its load.
     auto ready = [&](int ac) {
@@ -562,23 +509,12 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
         if (++sl == kF8Ring) sl = 0;
       }
     };
-    Tile next = first_tile();
-    int4 ahead = tile_rows(next.mi);
-    for (; next.i < ntiles; par ^= 1) {
-      const int ni = next.ni;
-      const int4 g = ahead;
-      next = next_tile(next);
-      ahead = tile_rows(next.mi);
-      const int pos0 = g.y + static_cast<int>(rank) * kF8Rows;
-      const int rows = g.z - static_cast<int>(rank) * kF8Rows;  // of this CTA; may be <= 0
-      const bool live = row < rows, warp_live = warp_row < rows;
-      int64_t o = -1;  // where this thread's row of outputs begins
-      if (MODE == kFp8Linear && live) o = static_cast<int64_t>(pos0 + row) * a.out_stride;
-      if (MODE == kFp8Down && live) {
-        const int slot = __ldcg(a.sorted + pos0 + row);
-        const int t = slot / a.s;
-        o = t * a.out_stride + (slot - t * a.s) * a.out_stride_s;
-      }
+    for (Tile t = first_tile(); t.i < ntiles; t = next_tile(t)) {
+      const int row0 = t.mi * kF8PairRows + static_cast<int>(rank) * kF8Rows;
+      const int rows = a.m - row0;  // of this CTA; may be <= 0
+      const bool warp_live = warp_row < rows;
+      // where this thread's row of outputs begins
+      const int64_t o = row < rows ? static_cast<int64_t>(row0 + row) * a.out_stride : -1;
       float acc[2][2][32];  // [col0, col1][half of the k-block's accumulators][column]
 #pragma unroll
       for (int j = 0; j < 32; ++j) acc[0][0][j] = acc[0][1][j] = acc[1][0][j] = acc[1][1][j] = 0.f;
@@ -587,13 +523,12 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
         // accumulator's first 32 columns behind this one's, the last 32 behind those.
         uint32_t v0[32], v1[32];
         const float2* fr = ring + row;
-        float2 f, fn = make_float2(0.f, 0.f);
+        float f, fn = 0.f;
         ready(2 * buf);
         auto factors = [&](int kb) {
-          float2 t = fr[(sl * kF8Group + (kb & (kF8Group - 1))) * kF8Rows];
-          if (MODE != kFp8GateUp) t.x = t.y = part ? t.y : t.x;  // one weight block
+          const float2 both = fr[(sl * kF8Group + (kb & (kF8Group - 1))) * kF8Rows];
           group_read(kb);
-          return t;
+          return part ? both.y : both.x;  // one weight block
         };
         f = factors(0);
         f8_ld32(lane_base + 2 * buf * kF8AccCols + col0, v0);
@@ -603,22 +538,22 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
           f8_ld_wait(v0);
           f8_ld_wait(v1);
           release(2 * buf);
-          f8_accumulate(acc[0][0], v0, f.x);
+          f8_accumulate(acc[0][0], v0, f);
           ready(2 * buf + 1);
           f8_ld32(d + kF8AccCols + col0, v0);
           const bool more = kb + 1 < kblocks;
           if (more) fn = factors(kb + 1);
-          f8_accumulate(acc[1][0], v1, f.y);
+          f8_accumulate(acc[1][0], v1, f);
           f8_ld32(d + kF8AccCols + col1, v1);
           f8_ld_wait(v0);
           f8_ld_wait(v1);
           release(2 * buf + 1);
-          f8_accumulate(acc[0][1], v0, f.x);
+          f8_accumulate(acc[0][1], v0, f);
           if (more) {
             ready(2 * (buf ^ 1));
             f8_ld32(dn + col0, v0);
           }
-          f8_accumulate(acc[1][1], v1, f.y);
+          f8_accumulate(acc[1][1], v1, f);
           if (more) f8_ld32(dn + col1, v1);
           f = fn;
           buf ^= 1;
@@ -633,53 +568,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
           group_read(kb);
         }
       }
-      if constexpr (MODE == kFp8GateUp) {
-        uint32_t m = 0;
-        if (warp_live) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {  // columns past I have zero weights: h = 0
-              acc[0][h][j] = silu_mul(acc[0][h][j], acc[1][h][j]);
-              m = max(m, abs_bits(acc[0][h][j]));
-            }
-        }
-        s_max[par][part][row] = __uint_as_float(m);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(maxima);
-        if (!*abort_flag) wait(maxima, 0, par);
-        m = max(m, __float_as_uint(s_max[par][part ^ 1][row]));
-        const float am = fp8_amax(m);
-        const float f = kE4m3Max / am;
-        __syncwarp();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float (&v)[32] = acc[0][h];
-#pragma unroll
-          for (int j = 0; j < 32; j += 16) {
-            uint4 q;
-            q.x = e4m3x4(v[j] * f, v[j + 1] * f, v[j + 2] * f, v[j + 3] * f);
-            q.y = e4m3x4(v[j + 4] * f, v[j + 5] * f, v[j + 6] * f, v[j + 7] * f);
-            q.z = e4m3x4(v[j + 8] * f, v[j + 9] * f, v[j + 10] * f, v[j + 11] * f);
-            q.w = e4m3x4(v[j + 12] * f, v[j + 13] * f, v[j + 14] * f, v[j + 15] * f);
-            *reinterpret_cast<uint4*>(buf_out + f8_unit(lane, 2 * h + j / 16)) = q;
-          }
-        }
-        __syncwarp();
-        // units 0, 1: this part's 32 of the low 64 columns, 2, 3: of the high ones; 8 rows at a time
-        uint8_t* dst = a.hq + static_cast<int64_t>(pos0 + warp_row) * f8_row_pitch(a.n) + ni * kFp8Block + part * 32 +
-                       ((lane & 3) >> 1) * 64 + (lane & 1) * 16;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 8 * i + (lane >> 2);
-          if (warp_row + r < rows)
-            *reinterpret_cast<uint4*>(dst + r * f8_row_pitch(a.n)) =
-                *reinterpret_cast<const uint4*>(buf_out + f8_unit(r, lane & 3));
-        }
-        if (live && part == 0) a.hs[ni * a.scale_rows + pos0 + row] = am / kE4m3Max;
-      } else if (warp_live) {
-        f8_store_rows(a.out, o, acc, (2 * ni + part) * kFp8Block, a.n, a.out_dtype, a.out_vec, buf_out);
-      }
+      if (warp_live) f8_store_rows(a.out, o, acc, (2 * t.ni + part) * kFp8Block, a.n, a.out_dtype, a.out_vec, buf_out);
     }
   }
 
@@ -825,7 +714,7 @@ __global__ void __launch_bounds__(256, kF8RowCtas) k_fp8_rows(F8PrepArgs a) {
 // counts its share per expert in shared memory; after a cluster barrier every CTA knows the counts
 // before its own (distributed shared memory) and places its slots, in any order within an expert (a
 // row's result does not depend on its place). groups[i] = (expert, first position, rows <=
-// group_rows, 0). One CTA took 42 us for 32768 slots.
+// group_rows (a multiple of 16), 0), an expert's as equal as steps of 16 allow. One CTA took 42 us for 32768 slots.
 constexpr int kF8PlanThreads = 1024;
 constexpr int kF8PlanCtas = 8;
 
@@ -853,7 +742,7 @@ __global__ void __launch_bounds__(kF8PlanThreads) __cluster_dims__(kF8PlanCtas, 
   if (bad && r.err) atomicOr(r.err, static_cast<uint32_t>(kErrBadExpert));
   cluster.sync();
   // Exclusive prefix of (slots, groups) over the experts, two consecutive experts per thread.
-  int c[2], g[2], mine[2];  // mine: slots of the CTAs before this one
+  int c[2], g[2], per[2], mine[2];  // mine: slots of the CTAs before this one
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int e = 2 * tid + j;
@@ -867,6 +756,7 @@ __global__ void __launch_bounds__(kF8PlanThreads) __cluster_dims__(kF8PlanCtas, 
       }
     }
     g[j] = (c[j] + group_rows - 1) / group_rows;
+    per[j] = g[j] ? ((c[j] + g[j] - 1) / g[j] + 15) / 16 * 16 : 0;  // equal groups, in steps of 16 rows
   }
   int sc = c[0] + c[1], sg = g[0] + g[1];
 #pragma unroll
@@ -896,7 +786,7 @@ __global__ void __launch_bounds__(kF8PlanThreads) __cluster_dims__(kF8PlanCtas, 
       next[e] = pos + mine[j];
       if (rank == 0)
         for (int k = 0; k < g[j]; ++k)
-          groups[gi + k] = make_int4(e, pos + k * group_rows, min(group_rows, c[j] - k * group_rows), 0);
+          groups[gi + k] = make_int4(e, pos + k * per[j], min(per[j], c[j] - k * per[j]), 0);
     }
     pos += c[j];
     gi += g[j];
