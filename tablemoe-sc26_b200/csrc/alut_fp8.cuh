@@ -164,26 +164,29 @@ constexpr int kFp8MaxExperts = 2048;  // two per thread of the plan
 
 // ---- the weight-streaming product ---------------------------------------------------------------
 //
-// For few rows per weight the time is the weights' way from HBM. A CTA takes 8 rows of x (the
-// N of mma.sync m16n8k32, weights as the M operand) and a slice of weight rows, in steps of
-// two 16-row tiles per warp, which are the gate and the up rows of 16 hidden units, or 32 adjacent
-// output columns. The eight warps are 8 / ks row groups; the ks warps of a group split K by blocks of
-// 128 and add up through shared memory in warp order: ks = 8 where few CTAs have to hide the latency
-// of one token, less where there are enough (fewer barriers per byte).
+// For few rows the time is the weights' way from HBM. A CTA takes 8 rows of x (the N of mma.sync
+// m16n8k32, weights as the M operand) and a slice of weight rows, in steps of two 16-row tiles per
+// warp, which are the gate and the up rows of 16 hidden units, or 32 adjacent output columns. The
+// eight warps are 8 / ks row groups; the ks warps of a group split K by blocks of 128 and add up
+// through shared memory in warp order: ks = 8 where few CTAs have to hide the latency of one token,
+// less where there are enough (fewer barriers per byte).
 // The weights come by 16-byte asynchronous copies into a ring in shared memory, kStreamDepth steps
-// ahead: 64 KB in flight per CTA, two CTAs per SM, where registers held a quarter of that (and the
-// decode step of 128 experts took 194 us instead of DECODE_US). Every lane copies the 16 bytes that it
-// reads itself (4 lanes a row, both 64-byte halves of a block), so the ring needs no barrier; and
-// since a dot product may be taken in any order of k, those words are used as they lie, x's in the
-// same order. x is quantised once per CTA, by the warp that needs the block: lane (g, c) holds 32
-// of row g's 128 columns, four lanes agree on the maximum, the words wait in shared memory.
-// The slots of an expert are served 8 at a time; a group's first slot leads (no plan pass).
+// ahead: 64 KB in flight per CTA, two CTAs per SM (registers held a quarter of that). Every lane
+// copies the 16 bytes that it reads itself (4 lanes a row, both 64-byte halves of a block), so the
+// ring needs no barrier; and since a dot product may be taken in any order of k, those words are used
+// as they lie, x's in the same order. x is quantised once per CTA, by the warp that needs the block:
+// lane (g, c) holds 32 of row g's 128 columns, four lanes agree on the maximum, the words wait in
+// shared memory. Up to 8 routed slots need no plan: an expert's first slot leads.
+// Measured, weights from HBM, one row: 2048 x 2048 5.6 us, 4096 x 4096 10.2, 150000 x 2048 58 (5.3
+// TB/s); 8 slots of 8 experts of 2048 x 768 (38 MB, two launches) 24.6. The small ones are bound by
+// latency: launch, x's form, the first weights, the reduction over warps.
 
 constexpr int kStreamRows = 8;        // rows of x per CTA
 constexpr int kStreamWRows = 16;      // weight rows per tile, two tiles per step
 constexpr int kStreamWarps = 8;
 constexpr int kStreamMaxSteps = 3;    // steps per CTA
-constexpr int kStreamMaxSlots = 512;  // slots a leader search looks through
+constexpr int kStreamMaxSlots = 8;    // routed slots of a call (its rule: experts_stream)
+static_assert(kStreamMaxSlots <= kStreamRows, "an expert's slots are one CTA's rows");
 constexpr int kStreamMaxBlocks = 64;  // of 128 columns: x's words in shared memory take 1 KB each
 constexpr int kStreamDepth = 2;       // steps' weights in flight per warp
 constexpr int kStreamStepUnits = 8 * 32;  // 16-byte units of a warp's step: [tile][row g, g + 8][64-byte half][lane]
@@ -283,20 +286,11 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 2) k_fp8_stream(StreamArgs 
     member = y * kStreamRows + lane;
   } else {
     const int n = a.r.q * a.r.s;
-    int ids[kStreamMaxSlots / 32];  // the slots' experts, all loads at once
     bool bad = false;
-#pragma unroll
-    for (int i = 0; i < kStreamMaxSlots / 32; ++i) {
-      bool ignored = false;
-      ids[i] = 32 * i + lane < n ? fp8_slot_expert(a.r, 32 * i + lane, ignored) : -1;
-      bad |= ignored && 32 * i + lane == y;
-    }
-    if (bad && a.r.err && warp == 0 && slice == 0) atomicOr(a.r.err, static_cast<uint32_t>(kErrBadExpert));
-    int mine = -1;
-#pragma unroll
-    for (int i = 0; i < kStreamMaxSlots / 32; ++i)
-      if (i == y >> 5) mine = __shfl_sync(kAll, ids[i], y & 31);
-    if (mine < 0) {
+    const int id = lane < n ? fp8_slot_expert(a.r, lane, bad) : -1;
+    if (bad && lane == y && a.r.err && warp == 0 && slice == 0) atomicOr(a.r.err, static_cast<uint32_t>(kErrBadExpert));
+    expert = __shfl_sync(kAll, id, y);
+    if (expert < 0) {
       if (MODE == kFp8Down && a.zero_skipped) {
         const int64_t o = static_cast<int64_t>(y / a.r.s) * a.out_stride + (y % a.r.s) * a.out_stride_s;
         const int c0 = slice * a.steps * groups * kStepRows, c1 = min(a.n, c0 + a.steps * groups * kStepRows);
@@ -304,24 +298,10 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 2) k_fp8_stream(StreamArgs 
       }
       return;
     }
-    expert = mine;
-    int before = 0;
-    cnt = 0;
-#pragma unroll
-    for (int i = 0; i < kStreamMaxSlots / 32; ++i) {
-      if (32 * i >= n || cnt == kStreamRows) continue;
-      unsigned hits = __ballot_sync(kAll, ids[i] == mine);
-      if (32 * i <= y) {
-        const unsigned below = y - 32 * i < 32 ? (1u << (y - 32 * i)) - 1u : kAll;
-        before += __popc(hits & below);
-        hits &= ~below;
-      }
-      // lane m takes the (m - cnt)-th of them
-      const unsigned mine_bit = __fns(hits, 0, lane - cnt + 1);
-      if (lane >= cnt && lane < kStreamRows && mine_bit < 32) member = 32 * i + mine_bit;
-      cnt = min(kStreamRows, cnt + __popc(hits));
-    }
-    if (before % kStreamRows) return;
+    const unsigned hits = __ballot_sync(kAll, id == expert);
+    if (hits & ((1u << y) - 1u)) return;  // an expert's first slot leads
+    cnt = __popc(hits);
+    if (lane < cnt) member = __fns(hits, 0, lane + 1);
   }
   const int all = groups * kStepRows;  // rows of a step
   const int r0 = slice * a.steps * all;

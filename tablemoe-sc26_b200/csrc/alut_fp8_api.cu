@@ -150,8 +150,21 @@ static int launch_rows(const F8PrepArgs& a, int x_dtype, cudaStream_t st) {
   return ALUT_OK;
 }
 
-// Which product a call takes: the weight-streaming one below these row counts.
-static bool linear_streams(int m, int k) { return m <= 16 && fp8_blocks(k) <= kStreamMaxBlocks; }
+// Which product a call takes. The streaming one reads the weights once per 8 rows, the tensor-core one
+// once (per 256), after a launch that writes x's 8-bit form. Measured (us, streaming / tensor cores,
+// weights from HBM): 2048 x 2048 5.6 / 12.7 for 1 row, 6.8 / 12.9 for 32, 12.0 / 14.7 for 64; 4096 x 4096
+// 10.2 / 18.7 for 1, 15.3 / 18.7 for 16, 21.7 / 18.8 for 24; 2560 x 2560 12.4 / 14.3 for 32, 15.3 / 16.7 for
+// 64; 12288 x 2048 12.2 / 13.9 for 8, 16.4 / 14.0 for 24; 150000 x 2048 61 / 83 for 8, 88 / 80 for 16: what is
+// read in all decides, and one pass is always streamed. Where that is little, the passes over x's form
+// do: 1024 x 1024 7.4 / 10.7 for 128, 10.4 / 10.7 for 192, 13.1 / 10.6 for 256; 2048 x 768 9.4 / 9.7 for 128,
+// 11.0 / 9.8 for 192.
+static bool linear_streams(int m, int n, int k) {
+  const int64_t passes = ceil_div(m, kStreamRows);
+  return (passes == 1 || (passes <= 16 && passes * n * k <= (40ll << 20))) && fp8_blocks(k) <= kStreamMaxBlocks;
+}
+// The same for routed slots, where the streaming kernels save the plan and the pass over x: 8 slots of
+// 128 experts of 2048 x 768 24.6 / 25.9 us, of 24 of 1000 x 600 17.2 / 20.0, of 8 of 2048 x 2816 34.0 / 31.8;
+// but 32 slots 51.9 / 47.3, 23.9 / 22.1, 50.5 / 45.1 and 128 slots 98 / 83, 35.5 / 25.8, 120 / 48.
 static bool experts_stream(const alut_fp8_experts_t* ex, int64_t slots) {
   return slots <= kStreamMaxSlots && fp8_blocks(std::max(ex->h, ex->i)) <= kStreamMaxBlocks;
 }
@@ -159,10 +172,10 @@ static bool experts_stream(const alut_fp8_experts_t* ex, int64_t slots) {
 struct LinearWorkspace {
   size_t xq, sx, total;
 };
-static LinearWorkspace linear_layout(int m, int k) {
+static LinearWorkspace linear_layout(int m, int n, int k) {
   LinearWorkspace w{};
   size_t off = 0;
-  if (!linear_streams(m, k)) {
+  if (!linear_streams(m, n, k)) {
     w.xq = off; off = align256(off + static_cast<size_t>(m) * f8_row_pitch(k));
     w.sx = off; off = align256(off + sizeof(float) * m * fp8_blocks(k));
   }
@@ -244,7 +257,7 @@ int alut_quantize_fp8(int64_t batch, int64_t rows, int32_t cols, int32_t block_r
 
 size_t alut_linear_fp8_workspace_size(int32_t m, int32_t n, int32_t k) {
   if (m < 0 || n <= 0 || k <= 0) return 0;
-  return linear_layout(m, k).total;
+  return linear_layout(m, n, k).total;
 }
 
 int alut_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, int32_t x_dtype, int64_t x_stride, const void* w,
@@ -261,9 +274,9 @@ int alut_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, int32_t x_dt
   if ((need && !workspace) || workspace_bytes < need)
     return fail(ALUT_EWORKSPACE, "linear_fp8: workspace has %zu bytes, needs %zu", workspace_bytes, need);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (!linear_streams(m, k)) {
+  if (!linear_streams(m, n, k)) {
     if (!aligned16(workspace)) return fail(ALUT_EWORKSPACE, "linear_fp8: workspace must be 16-byte aligned");
-    const LinearWorkspace ws = linear_layout(m, k);
+    const LinearWorkspace ws = linear_layout(m, n, k);
     char* base = static_cast<char*>(workspace);
     F8PrepArgs p{};
     p.x = x;

@@ -244,6 +244,48 @@ def test_experts_match_64_bits(q, s, e, h, i, keep, dtype):
     assert ex.device_errors() == 0
 
 
+@pytest.mark.parametrize("q,s,e", [(1, 8, 8), (1, 8, 40), (2, 4, 3), (8, 1, 2), (4, 2, 1), (1, 1, 5), (3, 2, 4)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_experts_of_few_slots(q, s, e, dtype):
+    g = gen(q + 10 * s + 100 * e)
+    h, i = 328, 200
+    weights, ex = make_experts(g, e, h, i)
+    x = activations(g, q, h, dtype)
+    sel = torch.randint(0, e, (q, s), generator=g, device=DEV)
+    comp = torch.rand(q, s, generator=g, device=DEV) < 0.7
+    out = ex(x, sel, comp)
+    check_experts(x, sel, comp, weights, out, dtype)
+    assert torch.equal(ex(x, sel)[comp], out[comp])  # whoever else shares the expert
+    assert ex.device_errors() == 0
+
+
+@pytest.mark.parametrize("m,n,k", [(128, 4096, 2688), (24, 4224, 4096), (16, 9000, 4480)])
+def test_linear_of_few_rows_and_much_weight(m, n, k):
+    g = gen(m)
+    x = activations(g, m, k, BF16)
+    w, s = weight(g, (), n, k)
+    want, bound = ref.product(ref.values(*ref.e4m3_form(x), 1), ref.values(w, s, 128))
+    close(Fp8Linear(w, s)(x), want, ref.with_output(want, bound, BF16), f"{m}x{n}x{k}")
+
+
+@pytest.mark.parametrize("h,i,dtype", [(256, 128, BF16), (200, 136, F16), (392, 260, F32)])
+def test_experts_with_any_number_of_tokens(h, i, dtype):
+    counts = [0, 1, 15, 16, 17, 33, 50, 64, 80, 96, 97, 112, 113, 127, 128, 129, 200, 257]
+    q = sum(counts)
+    g = gen(h)
+    weights, ex = make_experts(g, len(counts), h, i)
+    x = activations(g, q, h, dtype)
+    sel = torch.repeat_interleave(torch.arange(len(counts), device=DEV), torch.tensor(counts, device=DEV))
+    sel = sel[torch.randperm(q, generator=g, device=DEV)][:, None]
+    comp = torch.ones(q, 1, dtype=torch.bool, device=DEV)
+    out = ex(x, sel, comp)
+    check_experts(x, sel, comp, weights, out, dtype)
+    # a token's result does not depend on how many share its expert
+    few = torch.arange(0, q, 2, device=DEV)
+    assert torch.equal(out[few], ex(x[few], sel[few], comp[few]))
+    assert ex.device_errors() == 0
+
+
 @pytest.mark.parametrize("q", [12, 300])
 def test_experts_uneven_routing_and_empty_masks(q):
     g = gen(q)
