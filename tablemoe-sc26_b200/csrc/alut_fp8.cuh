@@ -254,10 +254,19 @@ __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// silu(g) u with the fast exponential and division: relative error about (4 + 1.2 |g|) 2^-23 (for
-// negative g, where exp(-g) counts), far under the e4m3 rounding that follows; the exact ones took
-// 16000 cycles a tile of the many-row product. exp(-g) = inf gives 0, silu's limit.
-__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
+// silu(g) u by the approximate exponential and reciprocal instructions: relative error about (4 + 1.2
+// |g|) 2^-23 (for negative g, where exp(-g) counts), far under the e4m3 rounding that follows; with the
+// exact ones a tile of the many-row product took 16000 cycles more. exp(-g) = inf gives 0, silu's limit.
+constexpr float kLog2E = 1.44269504f;
+__device__ __forceinline__ float exp2_approx(float x) {
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
+  return x;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(x));
+  return x;
+}
+__device__ __forceinline__ float silu_mul(float g, float u) { return g * rcp_approx(1.0f + exp2_approx(g * -kLog2E)) * u; }
 
 template <typename TX, int MODE>
 __global__ void __launch_bounds__(32 * kStreamWarps, 2) k_fp8_stream(StreamArgs a) {

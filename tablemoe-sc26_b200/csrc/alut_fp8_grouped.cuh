@@ -147,6 +147,23 @@ __device__ __forceinline__ uint64_t g8_fma(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+__device__ __forceinline__ uint64_t g8_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// silu_mul of both.
+__device__ __forceinline__ uint64_t g8_silu_mul(uint64_t g, uint64_t u) {
+  const float2 t = g8_unpair(g8_mul(g, g8_pair(-kLog2E, -kLog2E)));
+  const float2 e = g8_unpair(g8_add(g8_pair(exp2_approx(t.x), exp2_approx(t.y)), g8_pair(1.0f, 1.0f)));
+  return g8_mul(g8_mul(g, g8_pair(rcp_approx(e.x), rcp_approx(e.y))), u);
+}
+// The larger of m >= 0 and |x|; a NaN wins.
+__device__ __forceinline__ float g8_max_abs(float m, float x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
+  return r;
+}
 // Four (two) 8 x 8 matrices of 16-bit elements in that layout, stored transposed: lane 8 m + j gives the
 // address of the 16 bytes of matrix m's column j.
 __device__ __forceinline__ void g8_store_matrices(unsigned char* p, uint32_t m0, uint32_t m1, uint32_t m2, uint32_t m3) {
@@ -170,9 +187,11 @@ __device__ __forceinline__ uint32_t g8_pack(float lo, float hi) {
 }
 // A Down tile's outputs of one weight block: TMEM's rows are output columns (`n` left from `out` on),
 // its columns tokens, `tokens` of them there, whose outputs begin at off[]. acc[16-row half][8 tokens][..].
-template <typename TO, int C>
+// VEC: all 32 outputs are there, on 16 bytes. (The two cases are two loops, each short straight code: a
+// tile's end is bound by the instructions' way into the SM.)
+template <typename TO, bool VEC, int C>
 __device__ __forceinline__ void g8_store(TO* out, int n, const float (&acc)[2][C][4], const int64_t* off,
-                                         unsigned char (*stage)[kG8OutBytes], int tokens, int lane, bool vec) {
+                                         unsigned char (*stage)[kG8OutBytes], int tokens, int lane) {
   if constexpr (sizeof(TO) == 4) {
 #pragma unroll
     for (int i = 0; i < C * 8; ++i) {
@@ -195,7 +214,7 @@ __device__ __forceinline__ void g8_store(TO* out, int n, const float (&acc)[2][C
       const uint4 u = *reinterpret_cast<const uint4*>(buf + (lane / 4) * 80 + (lane & 3) * 16);
       if (t < tokens) {
         TO* p = out + off[t] + col;
-        if (vec && col + kVec <= n) {
+        if constexpr (VEC) {
           *reinterpret_cast<uint4*>(p) = u;
         } else {
           const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -509,26 +528,23 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         if (kBoth) add(b1, 0);
         add(b1, 1);
       }
-      float acc[2][2][C][4];  // [weight block][16-row half][8 tokens][2 row + token]
-#pragma unroll
-      for (int i = 0; i < 8 * C; ++i) {
-        const float2 t = g8_unpair(sum[i / (4 * C)][i / (2 * C) & 1][i / 2 % C][i & 1]);
-        float* p = &acc[i / (4 * C)][i / (2 * C) & 1][i / 2 % C][2 * (i & 1)];
-        p[0] = t.x;
-        p[1] = t.y;
-      }
       if constexpr (MODE == kFp8GateUp) {
         // h, and its maximum per token: over this lane's 4 rows, then over the 8 lanes of the same
         // tokens; in the first step a lane hands over the half that it does not keep.
-        uint32_t most[2 * C];  // [8 tokens][token]
+        float biggest[2 * C];  // [8 tokens][token]
 #pragma unroll
-        for (int i = 0; i < 8 * C; ++i) {  // rows past I have zero weights: h = 0
-          const int h = i / (4 * C), c = i / 4 % C;
-          float& v = acc[0][h][c][i & 3];
-          v = silu_mul(v, acc[1][h][c][i & 3]);
-          uint32_t& m = most[2 * c + (i & 1)];
-          m = h || (i & 2) ? max(m, abs_bits(v)) : abs_bits(v);
+        for (int i = 0; i < 4 * C; ++i) {  // rows past I have zero weights: h = 0
+          const int h = i / (2 * C), c = i / 2 % C;
+          uint64_t& v = sum[0][h][c][i & 1];
+          v = g8_silu_mul(v, sum[1][h][c][i & 1]);
+          const float2 t = g8_unpair(v);
+          float* m = &biggest[2 * c];
+          m[0] = g8_max_abs(h || (i & 1) ? m[0] : 0.f, t.x);
+          m[1] = g8_max_abs(h || (i & 1) ? m[1] : 0.f, t.y);
         }
+        uint32_t most[2 * C];
+#pragma unroll
+        for (int i = 0; i < 2 * C; ++i) most[i] = __float_as_uint(biggest[i]);
         // each lane of a pair hands over the half that it does not keep
         constexpr int kHalf = C % 2 == 0 ? C / 2 : C;  // kept after the second step (an odd C: everything)
         const bool up = lane & 16, up2 = C % 2 == 0 && (lane & 8);
@@ -568,8 +584,9 @@ __global__ void __launch_bounds__(kF8Threads, 1)
 #pragma unroll
           for (int i = 0; i < (c + 1 < C ? 4 : 2); ++i) {
             const float2 f = *reinterpret_cast<const float2*>(fac + (c + (i >> 1)) * 8 + 2 * (lane & 3));
-            const float(&u)[4] = acc[0][i & 1][c + (i >> 1)];
-            q[i] = e4m3x4(u[0] * f.x, u[2] * f.x, u[1] * f.y, u[3] * f.y);
+            const uint64_t(&u)[2] = sum[0][i & 1][c + (i >> 1)];
+            const float2 lo = g8_unpair(g8_mul(u[0], g8_pair(f.x, f.y))), hi = g8_unpair(g8_mul(u[1], g8_pair(f.x, f.y)));
+            q[i] = e4m3x4(lo.x, hi.x, lo.y, hi.y);
           }
           unsigned char* out = stage[c >> 1 & 1];
           if (c + 1 < C) g8_store_matrices(out + to, q[0], q[1], q[2], q[3]);
@@ -583,6 +600,14 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         }
         par ^= 1;
       } else {
+        float acc[2][2][C][4];  // [weight block][16-row half][8 tokens][2 row + token]
+  #pragma unroll
+        for (int i = 0; i < 8 * C; ++i) {
+          const float2 t = g8_unpair(sum[i / (4 * C)][i / (2 * C) & 1][i / 2 % C][i & 1]);
+          float* p = &acc[i / (4 * C)][i / (2 * C) & 1][i / 2 % C][2 * (i & 1)];
+          p[0] = t.x;
+          p[1] = t.y;
+        }
         int64_t* off = s_row[warp];
         __syncwarp();
 #pragma unroll
@@ -596,9 +621,15 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         for (int b = 0; b < 2; ++b) {
           const int col = (2 * ni + b) * kFp8Block + quarter * 32, n = a.n - col;
           if (n <= 0) continue;
-          if (a.out_dtype == ALUT_BF16) g8_store<__nv_bfloat16, C>(static_cast<__nv_bfloat16*>(a.out) + col, n, acc[b], off, stage, have, lane, a.out_vec);
-          else if (a.out_dtype == ALUT_F16) g8_store<__half, C>(static_cast<__half*>(a.out) + col, n, acc[b], off, stage, have, lane, a.out_vec);
-          else g8_store<float, C>(static_cast<float*>(a.out) + col, n, acc[b], off, stage, have, lane, false);
+          const bool vec = a.out_vec && n >= 32;
+          auto store = [&](auto* out) {
+            using TO = std::remove_pointer_t<decltype(out)>;
+            if (vec) g8_store<TO, true>(out + col, n, acc[b], off, stage, have, lane);
+            else g8_store<TO, false>(out + col, n, acc[b], off, stage, have, lane);
+          };
+          if (a.out_dtype == ALUT_BF16) store(static_cast<__nv_bfloat16*>(a.out));
+          else if (a.out_dtype == ALUT_F16) store(static_cast<__half*>(a.out));
+          else g8_store<float, false>(static_cast<float*>(a.out) + col, n, acc[b], off, stage, have, lane);
         }
       }
     };
