@@ -150,8 +150,8 @@ static int launch_rows(const F8PrepArgs& a, int x_dtype, cudaStream_t st) {
   return ALUT_OK;
 }
 
-// Which product a call takes. The streaming one reads the weights once per 8 rows, the tensor-core one
-// once (per 256), after a launch that writes x's 8-bit form. Measured (us, streaming / tensor cores,
+// Which product a call takes. The streaming one reads the weights once per 8 rows, the tensor-core ones
+// from L2 once per group, after a launch that writes x's 8-bit form. Measured (us, streaming / tensor cores,
 // weights from HBM): 2048 x 2048 5.6 / 12.7 for 1 row, 6.8 / 12.9 for 32, 12.0 / 14.7 for 64; 4096 x 4096
 // 10.2 / 18.7 for 1, 15.3 / 18.7 for 16, 21.7 / 18.8 for 24; 2560 x 2560 12.4 / 14.3 for 32, 15.3 / 16.7 for
 // 64; 12288 x 2048 12.2 / 13.9 for 8, 16.4 / 14.0 for 24; 150000 x 2048 61 / 83 for 8, 88 / 80 for 16: what is
@@ -161,6 +161,17 @@ static int launch_rows(const F8PrepArgs& a, int x_dtype, cudaStream_t st) {
 static bool linear_streams(int m, int n, int k) {
   const int64_t passes = ceil_div(m, kStreamRows);
   return (passes == 1 || (passes <= 16 && passes * n * k <= (40ll << 20))) && fp8_blocks(k) <= kStreamMaxBlocks;
+}
+// Tokens to a group of the grouped kernel, as few as still make one tile per SM; 0: pairs of CTAs, once
+// their tiles of 256 x 256 occupy about half the GPU. Measured (us, grouped / pairs): 2560 x 2560 14.2 /
+// 18.0 for 512 rows, 16.9 / 18.6 for 1024, 40.9 / 32.1 for 2048; 4096 x 4096 17.3 / 23.3 for 136, 20.5 / 24.2 for
+// 512, 26.2 / 24.8 for 768, 219 / 171 for 8192; 12288 x 2048 12.4 / 15.8 for 64, 17.1 / 16.7 for 256; 768 x
+// 2048 14.0 / 16.6 for 2048, 40.9 / 33.6 for 8192.
+static int linear_group(int m, int n) {
+  const int tiles = (fp8_blocks(n) + 1) / 2;
+  if (static_cast<int64_t>(ceil_div(m, kG8Tokens)) * tiles > 64) return 0;
+  const int groups = std::max(1, num_sms() / tiles);
+  return std::min<int>(kG8Tokens, static_cast<int>(round_up(ceil_div(m, groups), kG8Step)));
 }
 // The same for routed slots, where the streaming kernels save the plan and the pass over x: 8 slots of
 // 128 experts of 2048 x 768 24.6 / 25.9 us, of 24 of 1000 x 600 17.2 / 20.0, of 8 of 2048 x 2816 34.0 / 31.8;
@@ -288,8 +299,11 @@ int alut_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, int32_t x_dt
     p.sx = reinterpret_cast<float*>(base + ws.sx);
     p.scale_rows = m;
     CUtensorMap xm, wm;
-    rc = encode_rows(&xm, p.xq, m, k, kF8Rows);
-    if (!rc) {
+    const int group = linear_group(m, n);
+    rc = encode_rows(&xm, p.xq, m, k, group ? kG8Step : kF8Rows);
+    if (!rc && group) {
+      rc = encode_weight(&wm, w, k, n, 1, 1, w_stride, 0, 0);
+    } else if (!rc) {
       const uint64_t dims[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(n)}, strides[1] = {static_cast<uint64_t>(w_stride)};
       rc = encode_map(&wm, w, 2, dims, strides, kF8Rows);
     }
@@ -307,6 +321,8 @@ int alut_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, int32_t x_dt
     a.out_stride = out_stride;
     a.out_vec = rows_vec(out, out_stride, out_dtype);
     a.err = error_bits;
+    a.group = group;
+    if (group) return launch_grouped<kFp8Linear>(xm, wm, a, static_cast<int64_t>(ceil_div(m, group)) * ((fp8_blocks(n) + 1) / 2), st);
     return launch_tc(xm, wm, a, static_cast<int64_t>(ceil_div(m, kF8PairRows)) * ((fp8_blocks(n) + 1) / 2), st);
   }
   StreamArgs a{};

@@ -230,7 +230,6 @@ __device__ __forceinline__ void g8_store(TO* out, int n, const float (&acc)[2][C
 template <int MODE>
 __global__ void __launch_bounds__(kF8Threads, 1)
     k_fp8_grouped(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, F8Args a) {
-  static_assert(MODE == kFp8GateUp || MODE == kFp8Down, "grouped products");
   extern __shared__ unsigned char g8_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(g8_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem);  // [kG8Stages]
@@ -280,7 +279,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
   const uint32_t tmem = s_tmem;
   pdl_wait();  // the 8-bit rows, the plan and the scales come from the kernel before
   const int nt = MODE == kFp8GateUp ? nblocks : (nblocks + 1) / 2;  // tiles along the weight rows
-  const int mt = __ldcg(a.n_groups);
+  const int mt = MODE == kFp8Linear ? (a.m + a.group - 1) / a.group : __ldcg(a.n_groups);
   const int ntiles = mt * nt;  // (the host refuses more than fit)
   const int step = gridDim.x, step_m = step / nt, step_n = step % nt;
   struct Tile {  // walked without a division per tile: group mi, weight tile ni
@@ -298,7 +297,11 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     return t;
   };
   // A group: expert, first position, tokens. Every role reads its next tile's a tile ahead.
-  auto group_of = [&](int mi) { return mi < mt ? __ldcg(a.groups + mi) : make_int4(0, 0, 0, 0); };
+  auto group_of = [&](int mi) {
+    if (mi >= mt) return make_int4(0, 0, 0, 0);
+    if constexpr (MODE == kFp8Linear) return make_int4(0, mi * a.group, min(a.group, a.m - mi * a.group), 0);
+    else return __ldcg(a.groups + mi);
+  };
   auto wait = [&](uint64_t* bars, int i, uint32_t parity) {  // a fresh barrier counts as past parity 1
     f8_wait(smem_addr(bars) + 8 * i, parity, abort_flag, a.err);
   };
@@ -612,8 +615,12 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         __syncwarp();
 #pragma unroll
         for (int t = 0; t < (C > 4 ? 2 : 1); ++t) {
-          const int slot = t ? slots.y : slots.x, q = slot / a.s;
-          off[lane + 32 * t] = q * a.out_stride + (slot - q * a.s) * a.out_stride_s;
+          if constexpr (MODE == kFp8Linear) {
+            off[lane + 32 * t] = static_cast<int64_t>(g.y + hf * 8 * C + lane + 32 * t) * a.out_stride;
+          } else {
+            const int slot = t ? slots.y : slots.x, q = slot / a.s;
+            off[lane + 32 * t] = q * a.out_stride + (slot - q * a.s) * a.out_stride_s;
+          }
         }
         __syncwarp();
         const int have = min(tokens, 8 * C);

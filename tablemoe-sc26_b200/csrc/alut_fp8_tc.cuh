@@ -68,6 +68,7 @@ struct F8Args {
   int64_t scale_rows;       // rows (positions) in all
   const float* ws;          // weight scales, contiguous [E][halves][blocks n][blocks k]
   const int4* groups;       // GateUp, Down (alut_fp8_grouped.cuh): (expert, first position, rows, 0)
+  int group;                // Linear: tokens to a group, a multiple of 16
   const int* n_groups;
   const int* sorted;        // position -> slot
   int s;                    // slots per token

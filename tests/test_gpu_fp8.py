@@ -268,6 +268,29 @@ def test_linear_of_few_rows_and_much_weight(m, n, k):
     close(Fp8Linear(w, s)(x), want, ref.with_output(want, bound, BF16), f"{m}x{n}x{k}")
 
 
+@pytest.mark.parametrize("m,n,k", [(2600, 1100, 136), (1300, 1700, 264), (8200, 130, 1000), (1153, 1792, 640)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_linear_of_many_rows(m, n, k, dtype):
+    g = gen(m + n)
+    x = activations(g, m, k, dtype)
+    w, s = weight(g, (), n, k)
+    lin = Fp8Linear(w, s)
+    y = lin(x)
+    want, bound = ref.product(ref.values(*ref.e4m3_form(x), 1), ref.values(w, s, 128))
+    close(y, want, ref.with_output(want, bound, dtype), f"{m}x{n}x{k}")
+    buf = torch.full((m, n + 13), 7.0, dtype=dtype, device=DEV)
+    for off in (0, 5):
+        assert torch.equal(lin(x, out=buf[:, off:off + n]), y)
+        assert (buf[:, :off] == 7).all() and (buf[:, off + n:] == 7).all()
+        buf.fill_(7.0)
+    x[m // 2, 3], x[m - 1, 0] = float("nan"), float("inf")
+    z = lin(x)
+    assert not z[[m // 2, m - 1]].isfinite().any()
+    rest = torch.ones(m, dtype=torch.bool, device=DEV)
+    rest[[m // 2, m - 1]] = False
+    assert torch.equal(z[rest], y[rest]) and lin.device_errors() == 0
+
+
 @pytest.mark.parametrize("h,i,dtype", [(256, 128, BF16), (200, 136, F16), (392, 260, F32)])
 def test_experts_with_any_number_of_tokens(h, i, dtype):
     counts = [0, 1, 15, 16, 17, 33, 50, 64, 80, 96, 97, 112, 113, 127, 128, 129, 200, 257]
