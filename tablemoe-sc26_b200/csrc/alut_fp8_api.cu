@@ -36,7 +36,8 @@ static int launch_stream(StreamArgs a, int x_dtype, unsigned groups, bool pdl, c
   };
   // Few CTAs: every warp a share of K, the shortest way through. Enough for two per SM: at least 3
   // k-blocks a warp and up to kStreamMaxSteps steps per CTA, over which the search for the group and
-  // x's form are paid once.
+  // x's form are paid once. Measured, 8 rows: 32000 x 2048 19.2 us with this and 25.3 with all warps
+  // across K, 150000 x 2048 59 and 96 (71 with one step per CTA); up to 12288 x 2048 there is no difference.
   a.steps = 1;
   int ks = kStreamWarps;
   while (ks > kblocks) ks /= 2;

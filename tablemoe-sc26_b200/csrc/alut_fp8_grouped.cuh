@@ -1,11 +1,12 @@
-// The routed experts' block-scaled e4m3 products for many tokens: tcgen05 (kind::f8f6f4) with the
-// weights as the M operand and a group of tokens as N.
+// Block-scaled e4m3 products for tokens in groups: tcgen05 (kind::f8f6f4) with the weights as the M
+// operand and a group of tokens as N. The routed experts of more than 8 slots, and the plain product of
+// up to some hundred rows (one tile per SM: linear_group).
 //
 // An expert gets any number of tokens: 25 of a short prompt, 154 of a long one. With tokens as M (256
 // to a pair of CTAs) a tile costs 256 of them whether they are there or not; as N a group takes what it
 // has, in steps of 16 up to 128 (the plan cuts an expert's tokens into groups as equal as that allows).
 // A tile is two 128-row weight blocks x one group: the gate and the up rows of 128 hidden units
-// (GateUp), or 256 adjacent outputs (Down). Per 128 columns of K a CTA copies 32 KB of weights and 128
+// (GateUp), or 256 adjacent outputs (Down, Linear). Per 128 columns of K a CTA copies 32 KB of weights and 128
 // bytes a token. x's rows lie in the order of the plan (k_fp8_rows writes a token's 8-bit row once per
 // computed slot): gathering them here was slower (tile::gather4 moves a 128-byte row every 13 ns).
 // As in alut_fp8_tc.cuh an accumulator holds one k-block of one weight block (the scales change with
@@ -19,18 +20,21 @@
 //   warp 11    waits for accumulators and scales and lets the epilogue go by named barriers
 // TMEM is read 16 lanes x 8 columns at a time (16x256b): a thread has 4 weight rows of 2 tokens in each
 // 8, so that it needs a quarter of the group's scales. With a lane per row (32x32b) every sum needed
-// its own, and reading them (16 bytes per lane and 4 tokens) took most of the time: 182 + 146 us (GateUp
-// + Down) where this layout takes 134 + 100. The same fragments go out transposed by stmatrix, 32 to
-// 64 adjacent bytes of a token at a time.
+// its own, and reading them (16 bytes per lane and 4 tokens) took longer than anything else: 182 + 146
+// us (GateUp + Down of the first case below), 146 + 112 with this layout. The same fragments go out
+// transposed by stmatrix, 32 to 64 adjacent bytes of a token at a time. Sums, scales and silu are taken
+// two tokens at a time (f32x2): that, and a tile's end in less code, brought it to 136 + 93; a quarter
+// of the epilogue's time was the wait for instructions, of which each is used once per tile.
 // GateUp ends with h = silu(gate) up in its 8-bit form: the 128 rows of the tile are one block of the
 // next product, whose maximum per token is a reduction over 8 lanes and over the four quarters.
 //
-// Measured, 4096 tokens x 8 slots (60 % computed) over 128 experts of 2048 x 768: GateUp 134, Down
-// 100 us (with 256 tokens to a tile of a pair of CTAs 160 and 105); 300 x 6 over 72 experts of 2560 x
-// 1280: 89 and 55 us (130 and 75), 5.3 TB/s of weights. Copies and MMAs alone: 124 us together, and 105.
-// In the first the epilogue bounds it: 1200 cycles a k-block, 4700 of a tile's end during which the
-// MMAs run two k-blocks ahead at most. Sixteen epilogue warps instead of eight, with half the
-// accumulators each: 173 + 139. In the second, memory does.
+// Measured, 4096 tokens x 8 slots (60 % computed) over 128 experts of 2048 x 768: GateUp 136, Down 93
+// us (with 256 tokens to a tile of a pair of CTAs 160 and 105); 300 x 6 over 72 experts of 2560 x 1280:
+// 88 and 53 us (130 and 75), 5.4 and 4.5 TB/s of weights; 16 x 8 over the 128 experts 34 and 19 us.
+// Copies and MMAs alone take 124 us of the first pair, 105 of the second: 710 cycles a k-block for 80
+// tokens, the bytes through shared memory. In the first case the epilogue bounds it (1050 cycles a
+// k-block, and some 4000 of a tile's end during which the MMAs run two k-blocks ahead at most); sixteen
+// epilogue warps instead of eight, with half the sums each, took 173 + 139. In the others memory does.
 // Waits are bounded as in alut_fp8_tc.cuh.
 #pragma once
 

@@ -18,6 +18,8 @@
 // top-k is a local arg-max over NV registers and two warp reductions (redux.sync: largest
 // ordered key, then lowest expert id among equal keys). Latency-bound: a token's logits are
 // one or a few coalesced loads, the rest is the dependent chain of top_k + topk_group rounds.
+// Measured: 1 token of 128 experts, top 8: 3.0 us; 4096 of 256 in 8 groups (sigmoid, bias, two largest):
+// 12.8 us; 20011 of 72, biased softmax, top 6: 13.8 us (0.7 us of memory traffic each).
 #pragma once
 
 #include "alut_common.cuh"
