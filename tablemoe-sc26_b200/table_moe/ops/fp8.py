@@ -124,7 +124,10 @@ class Fp8Linear(_Fp8Module):
         v, xs, xd = self._check_x(x, self.k)
         m, n, k = v.shape[0], self.n, self.k
         if out is None:
-            y = torch.empty((*x.shape[:-1], n), dtype=out_dtype or x.dtype, device=self.device)
+            # (empty_strided takes 0.9 us less than empty)
+            y = torch.empty_strided((m, n), (n, 1), dtype=out_dtype or x.dtype, device=self.device)
+            if x.dim() != 2:
+                y = y.view(*x.shape[:-1], n)
             stride = n
         else:
             if out.shape != (m, n) or out.device != x.device or out.stride(-1) != 1:
@@ -134,7 +137,7 @@ class Fp8Linear(_Fp8Module):
             y, stride = out, out.stride(0) if m > 1 else max(out.stride(0), n)
         lib = self._lib
         nbytes = lib.alut_linear_fp8_workspace_size(m, n, k)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+        ws = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=self.device) if nbytes else None
         rc = lib.alut_linear_fp8(m, n, k, v.data_ptr(), xd, xs, self._w, self._w_stride, self._s, y.data_ptr(),
                                  _alut.dtype_code(y.dtype), stride, self._err, _alut.ptr(ws), nbytes,
                                  _alut.stream_ptr(self.device))
@@ -200,13 +203,13 @@ class Fp8Experts(_Fp8Module):
                 comp, comp_stride = comp.contiguous(), s
         out = collected
         if out is None:
-            out = torch.empty((q, s, h), dtype=x.dtype, device=dev)
+            out = torch.empty_strided((q, s, h), (s * h, h, 1), dtype=x.dtype, device=dev)
         elif out.shape != (q, s, h) or out.device != dev or out.stride(-1) != 1:
             raise ValueError(f"collected must be [{q}, {s}, {h}] on {dev} with unit innermost stride")
         out_t, out_s, _ = out.stride()
         lib = self._lib
         nbytes = lib.alut_experts_fp8_workspace_size(self._weights, q, s)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ws = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=dev)
         rc = lib.alut_experts_fp8(self._weights, q, s, v.data_ptr(), xd, xs, sel.data_ptr(), sel_stride, _alut.ptr(comp),
                                   comp_stride, 1 if collected is None else 0, out.data_ptr(),
                                   _alut.dtype_code(out.dtype), out_t, out_s, self._err, ws.data_ptr(), nbytes,
