@@ -1,6 +1,5 @@
 // 8-bit floating point (e4m3) products with a scale for each block of 128: the number form,
-// its quantisers, the plan that groups routed slots by expert, and the weight-streaming
-// product for few rows.
+// its quantisers, a routed slot's expert, and the weight-streaming product for few rows.
 //
 // The form. A row x is cut into blocks of 128 columns (the last one short). Per block, in
 // fp32: a = max(max|x|, 2^-100), scale s = a / 448, factor f = 448 / a, q = e4m3(x f) (round
@@ -41,11 +40,6 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 }
 
 // Runtime-typed element access (quantisers' inputs, ragged edges, outputs).
-__device__ __forceinline__ float load_any(const void* p, int64_t i, int dtype) {
-  if (dtype == ALUT_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-  if (dtype == ALUT_F16) return __half2float(static_cast<const __half*>(p)[i]);
-  return static_cast<const float*>(p)[i];
-}
 __device__ __forceinline__ void store_any(void* p, int64_t i, float v, int dtype) {
   if (dtype == ALUT_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
   else if (dtype == ALUT_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
@@ -56,77 +50,142 @@ __device__ __forceinline__ void store_any(void* p, int64_t i, float v, int dtype
 
 struct QuantArgs {
   int64_t batch, rows;
-  int cols, dtype;
+  int cols;
   const void* src;
   int64_t src_stride_b, src_stride;  // elements
   uint8_t* out;
   int64_t out_stride_b, out_stride;  // bytes
   float* scale;                       // contiguous [batch][row blocks][column blocks]
+  int src_vec, out_vec;               // rows start on 16 bytes, output rows on 8
 };
 
-// One scale per row and 128 columns: a warp per block, four consecutive columns per lane.
+// n / d by a 32-bit division where that holds both (64-bit ones take a microsecond each of a short call).
+__device__ __forceinline__ int64_t quant_div(int64_t n, int64_t d) {
+  return ((n | d) >> 32) == 0 ? static_cast<uint32_t>(n) / static_cast<uint32_t>(d) : n / d;
+}
+template <typename TX>
+struct F8Raw8 {  // 8 elements as they lie
+  uint4 w[sizeof(TX) / 2];
+};
+template <typename TX>
+__device__ __forceinline__ void f8_widen(const F8Raw8<TX>& r, float (&v)[8]) {
+  const TX* e = reinterpret_cast<const TX*>(&r);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = to_f32<TX>(e[j]);
+}
+// 8 columns of a row, zero from `left` on; and their 8-bit form, as many as there are.
+template <typename TX>
+__device__ __forceinline__ void quant_load8(const TX* p, int64_t left, bool vec, F8Raw8<TX>& v) {
+  if (vec && left >= 8) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(TX) / 2); ++i) v.w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    return;
+  }
+  TX* e = reinterpret_cast<TX*>(&v);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) e[j] = j < left ? p[j] : from_f32<TX>(0.f);
+}
+__device__ __forceinline__ void quant_store8(uint8_t* p, int64_t left, bool vec, const float (&v)[8], float f) {
+  const uint2 q = make_uint2(e4m3x4(v[0] * f, v[1] * f, v[2] * f, v[3] * f), e4m3x4(v[4] * f, v[5] * f, v[6] * f, v[7] * f));
+  if (vec && left >= 8) {
+    *reinterpret_cast<uint2*>(p) = q;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < left) p[j] = static_cast<uint8_t>((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
+}
+
+// One scale per row and 128 columns. Memory-bound: a warp takes 4 blocks of a row, two side by side (16
+// lanes of 8 columns each), all loads before the first maximum. 8192 x 4096 bf16: 30 us (3.3 TB/s); with
+// 2 blocks 34, with 8 40; 16 x 4096: 2.2 us, 2.0, 3.2.
+constexpr int kQuantBlocks = 4;
+template <typename TX>
 __global__ void __launch_bounds__(256) k_fp8_quantize_rows(QuantArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int kb = fp8_blocks(a.cols);
-  const int64_t n = a.batch * a.rows * kb;
+  const int lane = threadIdx.x & 31, sub = lane & 15, side = lane >> 4;
+  const int kb = fp8_blocks(a.cols), chunks = (kb + kQuantBlocks - 1) / kQuantBlocks;
+  const int64_t n = a.batch * a.rows * chunks;
   for (int64_t i = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; i < n;
        i += (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5) {
-    const int b = static_cast<int>(i % kb);
-    const int64_t row = i / kb;
-    const int64_t so = (row / a.rows) * a.src_stride_b + (row % a.rows) * a.src_stride;
-    const int64_t oo = (row / a.rows) * a.out_stride_b + (row % a.rows) * a.out_stride;
-    const int c0 = b * kFp8Block + lane * 4;
-    float v[4];
-    uint32_t m = 0;
+    const int64_t row = quant_div(i, chunks), bi = quant_div(row, a.rows), r = row - bi * a.rows;
+    const int b0 = static_cast<int>(i - row * chunks) * kQuantBlocks + side;
+    const int64_t c0 = static_cast<int64_t>(b0) * kFp8Block + sub * 8;
+    const TX* src = static_cast<const TX*>(a.src) + bi * a.src_stride_b + r * a.src_stride + c0;
+    uint8_t* out = a.out + bi * a.out_stride_b + r * a.out_stride + c0;
+    F8Raw8<TX> raw[kQuantBlocks / 2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[j] = c0 + j < a.cols ? load_any(a.src, so + c0 + j, a.dtype) : 0.f;
-      m = max(m, abs_bits(v[j]));
+    for (int u = 0; u < kQuantBlocks / 2; ++u)
+      quant_load8<TX>(src + 2 * u * kFp8Block, a.cols - c0 - 2 * u * kFp8Block, a.src_vec, raw[u]);
+#pragma unroll
+    for (int u = 0; u < kQuantBlocks / 2; ++u) {
+      float v[8];
+      f8_widen<TX>(raw[u], v);
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j]));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      if (b0 + 2 * u >= kb) continue;
+      const float am = fp8_amax(m);
+      quant_store8(out + 2 * u * kFp8Block, a.cols - c0 - 2 * u * kFp8Block, a.out_vec, v, kE4m3Max / am);
+      if (sub == 0) a.scale[row * kb + b0 + 2 * u] = am / kE4m3Max;
     }
-    const float am = fp8_amax(__reduce_max_sync(0xffffffffu, m));
-    const float f = kE4m3Max / am;
-    const uint32_t q = e4m3x4(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (c0 + j < a.cols) a.out[oo + c0 + j] = static_cast<uint8_t>(q >> (8 * j));
-    if (lane == 0) a.scale[i] = am / kE4m3Max;
   }
 }
 
-// One scale per 128 x 128 block (weights): a CTA per block.
-__global__ void __launch_bounds__(256) k_fp8_quantize_blocks(QuantArgs a) {
-  __shared__ uint32_t s_max;
+// One scale per 128 x 128 block (weights): a CTA per block, which stays in registers between its
+// maximum and its form. Four CTAs per SM, that some load while others convert: 128 x 1536 x 2048 bf16 423
+// us (2.9 TB/s), with two (119 registers, none spilled) 551, with six 679.
+template <typename TX>
+__global__ void __launch_bounds__(256, sizeof(TX) == 2 ? 4 : 3) k_fp8_quantize_blocks(QuantArgs a) {
+  __shared__ uint32_t s_max[2];
   const int kb = fp8_blocks(a.cols);
   const int64_t rb = (a.rows + kFp8Block - 1) / kFp8Block;
   const int64_t n = a.batch * rb * kb;
-  for (int64_t i = blockIdx.x; i < n; i += gridDim.x) {
-    const int64_t bi = i / (rb * kb), ri = (i / kb) % rb;
-    const int ci = static_cast<int>(i % kb);
+  constexpr int kU = kFp8Block * kFp8Block / 8 / 256;
+  const int c = (threadIdx.x & 15) * 8, rt = threadIdx.x >> 4;  // rows rt, rt + 16, ...
+  if (threadIdx.x < 2) s_max[threadIdx.x] = 0;
+  __syncthreads();
+  int turn = 0;
+  for (int64_t i = blockIdx.x; i < n; i += gridDim.x, turn ^= 1) {
+    const int64_t br = quant_div(i, kb), bi = quant_div(br, rb), ri = br - bi * rb;
+    const int ci = static_cast<int>(i - br * kb);
     const int64_t r0 = ri * kFp8Block;
     const int nr = static_cast<int>(min(static_cast<int64_t>(kFp8Block), a.rows - r0));
     const int nc = min(kFp8Block, a.cols - ci * kFp8Block);
-    const int64_t so = bi * a.src_stride_b + r0 * a.src_stride + ci * kFp8Block;
-    const int64_t oo = bi * a.out_stride_b + r0 * a.out_stride + ci * kFp8Block;
-    if (threadIdx.x == 0) s_max = 0;
-    __syncthreads();
+    const TX* src = static_cast<const TX*>(a.src) + bi * a.src_stride_b + r0 * a.src_stride + ci * kFp8Block + c;
+    uint8_t* out = a.out + bi * a.out_stride_b + r0 * a.out_stride + ci * kFp8Block + c;
+    F8Raw8<TX> raw[kU];
     uint32_t m = 0;
-    for (int e = threadIdx.x; e < kFp8Block * kFp8Block; e += blockDim.x) {
-      const int r = e >> 7, c = e & 127;
-      if (r < nr && c < nc) m = max(m, abs_bits(load_any(a.src, so + r * a.src_stride + c, a.dtype)));
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int r = rt + 16 * u;
+      quant_load8<TX>(src + r * a.src_stride, r < nr ? nc - c : 0, a.src_vec, raw[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      float v[8];
+      f8_widen<TX>(raw[u], v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j]));
     }
     m = __reduce_max_sync(0xffffffffu, m);
-    if ((threadIdx.x & 31) == 0) atomicMax(&s_max, m);
+    if ((threadIdx.x & 31) == 0) atomicMax(&s_max[turn], m);
     __syncthreads();
-    const float am = fp8_amax(s_max);
+    const float am = fp8_amax(s_max[turn]);
     const float f = kE4m3Max / am;
-    for (int e = threadIdx.x; e < kFp8Block * kFp8Block; e += blockDim.x) {
-      const int r = e >> 7, c = e & 127;
-      if (r < nr && c < nc)
-        a.out[oo + r * a.out_stride + c] =
-            static_cast<uint8_t>(e4m3x2(load_any(a.src, so + r * a.src_stride + c, a.dtype) * f, 0.f));
+    if (threadIdx.x == 0) {
+      s_max[turn ^ 1] = 0;  // the next block's; read last before this barrier
+      a.scale[i] = am / kE4m3Max;
     }
-    if (threadIdx.x == 0) a.scale[i] = am / kE4m3Max;
-    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int r = rt + 16 * u;
+      float v[8];
+      f8_widen<TX>(raw[u], v);
+      if (r < nr) quant_store8(out + r * a.out_stride, nc - c, a.out_vec, v, f);
+    }
+    __syncthreads();  // (the cleared maximum)
   }
 }
 

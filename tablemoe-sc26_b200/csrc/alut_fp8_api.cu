@@ -253,17 +253,23 @@ int alut_quantize_fp8(int64_t batch, int64_t rows, int32_t cols, int32_t block_r
   if (batch == 0 || rows == 0 || cols == 0) return ALUT_OK;
   if (!src || !out || !scale) return fail(ALUT_EINVAL, "quantize_fp8: NULL argument");
   if (src_stride < cols || out_stride < cols) return fail(ALUT_ESHAPE, "quantize_fp8: row strides");
-  QuantArgs a{batch, rows, cols, dtype, src, src_stride_b, src_stride, static_cast<uint8_t*>(out), out_stride_b,
+  QuantArgs a{batch, rows, cols, src, src_stride_b, src_stride, static_cast<uint8_t*>(out), out_stride_b,
               out_stride, scale};
+  a.src_vec = rows_vec(src, src_stride, dtype) && rows_vec(src, src_stride_b, dtype);
+  a.out_vec = (reinterpret_cast<uintptr_t>(out) | out_stride | out_stride_b) % 8 == 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int64_t kb = fp8_blocks(cols);
   if (block_rows == 1) {
-    const int64_t n = batch * rows * kb;
-    k_fp8_quantize_rows<<<static_cast<unsigned>(std::min<int64_t>((n + 7) / 8, 16 * num_sms())), 256, 0, st>>>(a);
+    const int64_t n = batch * rows * ((kb + kQuantBlocks - 1) / kQuantBlocks);
+    auto kern = dtype == ALUT_BF16 ? k_fp8_quantize_rows<__nv_bfloat16>
+                                   : dtype == ALUT_F16 ? k_fp8_quantize_rows<__half> : k_fp8_quantize_rows<float>;
+    kern<<<static_cast<unsigned>(std::min<int64_t>((n + 7) / 8, 16 * num_sms())), 256, 0, st>>>(a);
     return check_launch("k_fp8_quantize_rows");
   }
   const int64_t n = batch * ((rows + kFp8Block - 1) / kFp8Block) * kb;
-  k_fp8_quantize_blocks<<<static_cast<unsigned>(std::min<int64_t>(n, 1 << 20)), 256, 0, st>>>(a);
+  auto kern = dtype == ALUT_BF16 ? k_fp8_quantize_blocks<__nv_bfloat16>
+                                 : dtype == ALUT_F16 ? k_fp8_quantize_blocks<__half> : k_fp8_quantize_blocks<float>;
+  kern<<<static_cast<unsigned>(std::min<int64_t>(n, 1 << 20)), 256, 0, st>>>(a);
   return check_launch("k_fp8_quantize_blocks");
 }
 

@@ -610,16 +610,6 @@ struct F8PrepArgs {
 constexpr int kF8RowBlocks = 8;
 constexpr int kF8RowCtas = 4;  // per SM: 32 warps with 2 KB each on the way
 template <typename TX>
-struct F8Raw8 {  // 8 elements as they lie
-  uint4 w[sizeof(TX) / 2];
-};
-template <typename TX>
-__device__ __forceinline__ void f8_widen(const F8Raw8<TX>& r, float (&v)[8]) {
-  const TX* e = reinterpret_cast<const TX*>(&r);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = to_f32<TX>(e[j]);
-}
-template <typename TX>
 __global__ void __launch_bounds__(256, kF8RowCtas) k_fp8_rows(F8PrepArgs a) {
   constexpr int kU = kF8RowBlocks / 2;
   pdl_launch_dependents();
