@@ -309,6 +309,22 @@ def test_experts_with_any_number_of_tokens(h, i, dtype):
     assert ex.device_errors() == 0
 
 
+@pytest.mark.parametrize("h,i,dtype", [(256, 128, F16), (200, 136, F32), (1160, 520, BF16)])
+def test_experts_with_many_tokens_each(h, i, dtype):
+    counts = [700, 97, 112, 113, 128, 241, 0, 131]
+    q = sum(counts)
+    g = gen(h + 1)
+    weights, ex = make_experts(g, len(counts), h, i)
+    x = activations(g, q, h, dtype)
+    sel = torch.repeat_interleave(torch.arange(len(counts), device=DEV), torch.tensor(counts, device=DEV))
+    sel = sel[torch.randperm(q, generator=g, device=DEV)][:, None]
+    out = ex(x, sel)
+    check_experts(x, sel, torch.ones(q, 1, dtype=torch.bool, device=DEV), weights, out, dtype)
+    few = torch.arange(0, q, 4, device=DEV)  # other groups, the same results
+    assert torch.equal(out[few], ex(x[few], sel[few]))
+    assert ex.device_errors() == 0
+
+
 @pytest.mark.parametrize("q", [12, 300])
 def test_experts_uneven_routing_and_empty_masks(q):
     g = gen(q)
