@@ -6,8 +6,8 @@
 // to a pair of CTAs) a tile costs 256 of them whether they are there or not; as N a group takes what it
 // has, in steps of 16 up to 128 (the plan cuts an expert's tokens into groups as equal as that allows).
 // A tile is two 128-row weight blocks x one group: the gate and the up rows of 128 hidden units
-// (GateUp), or 256 adjacent outputs (Down, Linear). Per 128 columns of K a CTA copies 32 KB of weights and 128
-// bytes a token. x's rows lie in the order of the plan (k_fp8_rows writes a token's 8-bit row once per
+// (GateUp), or 256 adjacent outputs (Down, Linear). Per 128 columns of K a CTA copies 32 KB of weights
+// and 128 bytes a token. x's rows lie in the order of the plan (k_fp8_rows writes a token's 8-bit row once per
 // computed slot): gathering them here was slower (tile::gather4 moves a 128-byte row every 13 ns).
 // As in alut_fp8_tc.cuh an accumulator holds one k-block of one weight block (the scales change with
 // each): four of 128 columns in tensor memory, each added up, times sx[token, block] sw[block], in fp32
@@ -30,11 +30,12 @@
 //
 // Measured, 4096 tokens x 8 slots (60 % computed) over 128 experts of 2048 x 768: GateUp 136, Down 93
 // us (with 256 tokens to a tile of a pair of CTAs 160 and 105); 300 x 6 over 72 experts of 2560 x 1280:
-// 88 and 53 us (130 and 75), 5.4 and 4.5 TB/s of weights; 16 x 8 over the 128 experts 34 and 19 us.
-// Copies and MMAs alone take 124 us of the first pair, 105 of the second: 710 cycles a k-block for 80
-// tokens, the bytes through shared memory. In the first case the epilogue bounds it (1050 cycles a
-// k-block, and some 4000 of a tile's end during which the MMAs run two k-blocks ahead at most); sixteen
-// epilogue warps instead of eight, with half the sums each, took 173 + 139. In the others memory does.
+// 78 and 50 us (130 and 75), 6.1 and 4.7 TB/s of weights, with groups of up to 48 tokens (of up to 128:
+// 88 and 53); 16 x 8 over the 128 experts 36 and 20 us, 4.5 TB/s. Copies and MMAs alone take 124 us of
+// the first pair: 710 cycles a k-block for 80 tokens. In the first case the epilogue bounds it (1050
+// cycles a k-block, and some 4000 of a tile's end during which the MMAs run two k-blocks ahead at
+// most); sixteen epilogue warps instead of eight, with half the sums each, took 173 + 139. In the
+// others memory does.
 // Waits are bounded as in alut_fp8_tc.cuh.
 #pragma once
 
