@@ -338,7 +338,8 @@ size_t alut_route_workspace_size(int32_t num_experts);
 /* Top-k softmax routing and keep mask of q tokens in one call:
  *   probabilities = softmax(fp32(logits[t, :num_experts])) (logits f32/bf16/f16, row stride
  *   logits_stride); weights[t, s], sel[t, s] = the top_k largest in descending order (lower
- *   expert id first among equal probabilities); with normalize_topk the weights are divided
+ *   expert id first among equal probabilities; a row of only -inf has probabilities 0, one with
+ *   a NaN or a +inf NaN, and either names its lowest expert ids); with normalize_topk the weights are divided
  *   by max(their sum, 1e-20) (qwen_topk_softmax.py:150-151);
  *   compute[t, s] = 1 for computed slots, reuse[t, s] = 1 - compute[t, s] for looked-up ones:
  *     ALUT_KEEP_FIXED: s < keep_k;

@@ -4,7 +4,9 @@
 // Semantics (reference project fanyalun/tablemoe-sc26):
 //  * table_moe/ops/qwen_topk_softmax.py:122-153: probabilities = softmax(fp32 logits), the
 //    top_k largest in descending order (weights, expert ids); with normalize_topk the
-//    weights are divided by their sum clamped at 1e-20;
+//    weights are divided by their sum clamped at 1e-20. A row of only -inf (every expert
+//    masked out) has probabilities 0, a row with a NaN or a +inf has NaN everywhere; NaN
+//    ranks below every number, so both rows name their lowest expert ids;
 //  * table_moe/skip/pruning.py:4-15 build_fixed_keep_mask / :51 build_decode_keep_mask:
 //    the first keep_k slots of every token are computed (keep_k clamped to [0, top_k];
 //    "none" keeps every slot);
@@ -75,17 +77,19 @@ __global__ void __launch_bounds__(kRouteWarps * 32) k_route_topk(RouteArgs a) {
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  const float shift = mx == -INFINITY ? 0.f : mx;
   float sum = 0.f;
   for (int j = lane; j < a.e; j += 32) {
-    const float ex = expf(p[j] - mx);
+    const float ex = expf(p[j] - shift);
     p[j] = ex;
     sum += ex;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  for (int j = lane; j < a.e; j += 32) p[j] = p[j] / sum;
+  for (int j = lane; j < a.e; j += 32) p[j] = sum == 0.f ? 0.f : p[j] / sum;
   __syncwarp();
-  // top_k rounds of arg-max; the chosen entry is retired with -1 (probabilities are >= 0).
+  // top_k <= E rounds of arg-max; the chosen entry is retired with -1. Probabilities are >= 0 and
+  // a NaN counts as -0.5, so every round finds an entry that is not retired: bi is an expert's.
   __shared__ float s_w[kRouteWarps][kMaxSlots];
   __shared__ int s_i[kRouteWarps][kMaxSlots];
   for (int s = 0; s < a.k; ++s) {
@@ -93,8 +97,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32) k_route_topk(RouteArgs a) {
     int bi = 0x7fffffff;
     for (int j = lane; j < a.e; j += 32) {
       const float v = p[j];
-      if (v > bv) {  // ascending j per lane: the lane's first maximum is kept
-        bv = v;
+      const float key = isnan(v) ? -0.5f : v;
+      if (key > bv) {  // ascending j per lane: the lane's first maximum is kept
+        bv = key;
         bi = j;
       }
     }
@@ -108,9 +113,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32) k_route_topk(RouteArgs a) {
       }
     }
     if (lane == 0) {
-      p[bi] = -1.f;
-      s_w[warp][s] = bv;
+      s_w[warp][s] = p[bi];
       s_i[warp][s] = bi;
+      p[bi] = -1.f;
     }
     __syncwarp();
   }
@@ -119,7 +124,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) k_route_topk(RouteArgs a) {
     // Sum of the selected weights in slot order (the reference's weights.sum(dim=-1)),
     // clamped at 1e-20 (qwen_topk_softmax.py:151).
     for (int s = 0; s < a.k; ++s) tot += s_w[warp][s];
-    tot = fmaxf(tot, 1e-20f);
+    tot = fmaxf(tot, 1e-20f);  // (the sum of NaN weights too: they stay NaN)
   }
   for (int s = lane; s < a.k; s += 32) {
     float wv = s_w[warp][s];
