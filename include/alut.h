@@ -423,6 +423,12 @@ int alut_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, int32_t x_dt
                     int64_t w_stride, const float* w_scale, void* out, int32_t out_dtype, int64_t out_stride,
                     uint32_t* error_bits, void* workspace, size_t workspace_bytes, alut_stream_t stream);
 
+/* How long a wait inside the kernels of alut_linear_fp8 and alut_experts_fp8 (for a copy or for the
+ * tensor cores) may take, for this thread's calls from now on: 1e9 ns unless set. A call whose wait
+ * runs out sets ALUT_ERR_MMA_TIMEOUT in error_bits, ends, and leaves its output undefined. 0: calls
+ * give up before their first such wait (to test what handles the error). */
+int alut_set_wait_limit(uint64_t ns);
+
 /* The experts of a layer: down(silu(gate . x) * (up . x)). Weights e4m3 with the rules of
  * alut_linear_fp8; all strides are multiples of 16 bytes. */
 typedef struct alut_fp8_experts {
@@ -468,7 +474,7 @@ int alut_normalize_rows(int64_t rows, int32_t l, const void* src, int64_t src_st
  * first and has no counterpart of the others. */
 #define ALUT_ERR_BAD_EXPERT 1u  /* a searched slot's expert id is outside [0, num_experts) */
 #define ALUT_ERR_COPY_TIMEOUT 4u /* a key-chunk copy did not land within 1 s */
-#define ALUT_ERR_MMA_TIMEOUT 8u  /* a tensor-core pipeline wait ran out (1 s) */
+#define ALUT_ERR_MMA_TIMEOUT 8u  /* a tensor-core pipeline wait ran out (1 s, or alut_set_wait_limit) */
 int alut_workspace_errors(void* workspace, size_t workspace_bytes, int32_t clear, uint32_t* bits,
                           alut_stream_t stream);
 

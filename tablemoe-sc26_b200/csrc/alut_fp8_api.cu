@@ -9,6 +9,8 @@
 
 namespace alut {
 
+static thread_local uint64_t g_wait_ns = kWaitNs;  // alut_set_wait_limit
+
 static int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 // Checks shared by every e4m3 weight.
@@ -283,6 +285,11 @@ int alut_quantize_fp8(int64_t batch, int64_t rows, int32_t cols, int32_t block_r
   return check_launch("k_fp8_quantize_blocks");
 }
 
+int alut_set_wait_limit(uint64_t ns) {
+  g_wait_ns = ns;
+  return ALUT_OK;
+}
+
 size_t alut_linear_fp8_workspace_size(int32_t m, int32_t n, int32_t k) {
   if (m < 0 || n <= 0 || k <= 0) return 0;
   return linear_layout(m, n, k).total;
@@ -338,6 +345,7 @@ int alut_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, int32_t x_dt
     a.out_stride = out_stride;
     a.out_vec = rows_vec(out, out_stride, out_dtype);
     a.err = error_bits;
+    a.wait_ns = g_wait_ns;
     a.group = group;
     if (group) return launch_grouped<kFp8Linear>(xm, wm, a, static_cast<int64_t>(ceil_div(m, group)) * ((fp8_blocks(n) + 1) / 2), st);
     return launch_tc(xm, wm, a, static_cast<int64_t>(ceil_div(m, kF8PairRows)) * ((fp8_blocks(n) + 1) / 2), st);
@@ -429,6 +437,7 @@ int alut_experts_fp8(const alut_fp8_experts_t* ex, int32_t q, int32_t s, const v
     if (rc) return rc;
     a.s = s;
     a.err = error_bits;
+    a.wait_ns = g_wait_ns;
     a.n = ex->i;
     a.k = ex->h;
     a.sx = p.sx;

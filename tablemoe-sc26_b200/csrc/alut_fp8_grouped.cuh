@@ -36,7 +36,7 @@
 // cycles a k-block, and some 4000 of a tile's end during which the MMAs run two k-blocks ahead at
 // most); sixteen epilogue warps instead of eight, with half the sums each, took 173 + 139. In the
 // others memory does.
-// Waits are bounded as in alut_fp8_tc.cuh.
+// Waits are bounded, and an abort ends, as in alut_fp8_tc.cuh.
 #pragma once
 
 #include <type_traits>
@@ -276,7 +276,8 @@ __global__ void __launch_bounds__(kF8Threads, 1)
       mbar_init(&f_empty[i], kF8EpiWarps);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    s_abort = 0;
+    s_abort = a.wait_ns == 0;
+    if (a.wait_ns == 0 && a.err) atomicOr(a.err, static_cast<uint32_t>(kErrMmaTimeout));
   }
   tc_fence_before();
   __syncthreads();
@@ -308,7 +309,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     else return __ldcg(a.groups + mi);
   };
   auto wait = [&](uint64_t* bars, int i, uint32_t parity) {  // a fresh barrier counts as past parity 1
-    f8_wait(smem_addr(bars) + 8 * i, parity, abort_flag, a.err);
+    return f8_wait<false>(smem_addr(bars) + 8 * i, parity, abort_flag, a);
   };
   auto stopped = [&]() { return __any_sync(0xffffffffu, *abort_flag); };
 
@@ -328,7 +329,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         const int parts = (g.z + kG8Step - 1) / kG8Step;
         const uint32_t bytes = 2 * kF8TileBytes + parts * kG8Step * kFp8Block;
         for (int kb = 0; kb < kblocks; ++kb, (++st == kG8Stages ? (st = 0, past ^= 1) : 0)) {
-          wait(empty, st, past);
+          if (!wait(empty, st, past)) break;
           if (f8_elect()) {
             unsigned char* sw = stages + static_cast<size_t>(st) * kG8StageBytes;
             const int x = kb * kFp8Block;
@@ -360,11 +361,10 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         for (int kb = 0; kb < kblocks; ++kb) {
           const uint64_t dw = desc0 + static_cast<uint32_t>(st) * (kG8StageBytes >> 4), dx = dw + (2 * kF8TileBytes >> 4);
           const uint32_t d = tmem + 2 * buf * kF8AccCols, done = done0 + 16 * buf;
-          wait(full, st, ph);
-          wait(t_empty, 2 * buf, past);
+          if (!wait(full, st, ph) || !wait(t_empty, 2 * buf, past)) break;
           tc_fence_after();
           g8_issue<false>(d, dw, dx, idesc, done, 0);
-          wait(t_empty, 2 * buf + 1, past);
+          if (!wait(t_empty, 2 * buf + 1, past)) break;
           tc_fence_after();
           g8_issue<true>(d + kF8AccCols, dw + (kF8TileBytes >> 4), dx, idesc, done + 8, freed0 + 8 * st);
           if (++st == kG8Stages) {
@@ -430,29 +430,36 @@ __global__ void __launch_bounds__(kF8Threads, 1)
       }
     } else {
       // ---- accumulators (and their factors) done: let the epilogue go ------------------------------
-      // It and the epilogue run through every tile even after an abort, without waiting then: a
-      // named barrier's counts have to match.
       int sl = 0, sph = 0, buf = 0, ph = 0;
-      for (int tile = blockIdx.x; tile < ntiles; tile += step) {
-        for (int kb = 0; kb < kblocks; ++kb) {
+      uint32_t gone = 0;  // k-blocks of the tiles before this one
+      bool given_up = a.wait_ns == 0;
+      int kb = 0, b = 0;
+      for (int tile = blockIdx.x; tile < ntiles && !given_up; tile += step) {
+        for (kb = 0; kb < kblocks; ++kb) {
           if ((kb & (kF8Group - 1)) == 0) {
-            if (!*abort_flag) wait(f_full, sl, sph);
+            wait(f_full, sl, sph);
             if (++sl == kF8Ring) {
               sl = 0;
               sph ^= 1;
             }
           }
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            if (!*abort_flag) wait(t_full, 2 * buf + b, ph);
-            __syncwarp();
+          for (b = 0; b < 2; ++b) {
+            given_up = !wait(t_full, 2 * buf + b, ph);
+            if (given_up) break;
 #pragma unroll
             for (int p = 0; p < 2; ++p)
               asm volatile("bar.arrive %0, %1;" ::"r"(1 + kF8Acc * p + 2 * buf + b), "n"(32 * 5) : "memory");
           }
+          if (given_up) break;
           ph ^= buf;
           buf ^= 1;
         }
+        if (!given_up) gone += kblocks;
+      }
+      if (given_up) {
+        const uint32_t first = blockIdx.x, tiles = first < ntiles ? (ntiles - first + step - 1) / step : 0;
+        f8_drain<kF8Acc, 32 * 5>(smem_addr(t_empty), a.wait_ns == 0 ? 0 : 2 * (gone + kb) + b, 2 * tiles * kblocks);
       }
     }
   } else {

@@ -27,7 +27,9 @@
 // A thread ends with a row segment of 128 outputs, which goes out through shared memory so that a
 // store instruction writes 256 adjacent bytes of two rows (one bulk copy per row instead took 2400
 // cycles a warp to issue).
-// Every wait is bounded in time (error bit, stop, time for what is in flight, TMEM freed).
+// Every wait for a copy, an MMA or a factor is bounded in time (error bit, stop, time for what is in
+// flight, TMEM freed). The epilogue's named barriers need warp 11 alone, which goes through all of them
+// whatever has run out (f8_drain).
 // Measured: 8192 x 4096 x 4096 151 us with x's form (23 of them), 1.8 PFLOP/s; 4096 x 4096 x 4096 87; 2048 x
 // 2560 x 2560 32. Bound by the accumulators' way back to registers (about 1000 cycles a k-block).
 #pragma once
@@ -80,6 +82,7 @@ struct F8Args {
   int out_dtype, out_vec;   // out_vec: 16-byte stores are aligned
   int64_t out_stride, out_stride_s;
   uint32_t* err;
+  uint64_t wait_ns;         // how long a wait may take; 0: the call gives up before its first
 };
 
 // The same shared variable of the pair's CTA `rank`, as a shared::cluster address.
@@ -93,10 +96,6 @@ __device__ __forceinline__ uint32_t f8_of_rank(const void* p, uint32_t rank) {
 __device__ __forceinline__ void f8_arrive_remote(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// Waits on a barrier of this CTA (by its shared address). A wait that runs out (1 s), or that another
-// role has given up, returns as if it were over: the flag and the error bit say so, each role stops
-// at its next tile, and what it does until then stays in bounds. The timer is read only every 256
-// tries: a read of %globaltimer takes most of a microsecond.
 __device__ __forceinline__ bool f8_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -115,18 +114,63 @@ __device__ __forceinline__ bool f8_test(uint32_t bar, uint32_t parity) {  // a l
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ void f8_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t* err) {
+template <bool PAIR>
+__device__ __forceinline__ void f8_give_up(volatile int* abort_flag) {
+  *abort_flag = 1;
+  if constexpr (PAIR) {
+    uint32_t rank, there;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(smem_addr(const_cast<int*>(abort_flag))), "r"(rank ^ 1));
+    asm volatile("st.shared::cluster.u32 [%0], 1;\n fence.acq_rel.cluster;" ::"r"(there) : "memory");
+  }
+}
+// Waits of a whole warp on a barrier of this CTA (by its shared address); false: it ran out, or another
+// role has given up (the flag and the error bit say so). The copies and each role's next tile stop then,
+// and what is done until then stays in bounds. The timer is read only every 256 tries: a read of
+// %globaltimer takes most of a microsecond.
+// What must not happen is that warp 11 takes an accumulator for full that was filled out of turn, while
+// the epilogue has yet to pass that barrier's last use (f8_drain says why).
+//   One CTA: the lanes agree on the answer by a vote, and the MMA warp stops where one of its waits fails,
+//   so no accumulator is filled out of turn before warp 11 itself has given up.
+//   PAIR: the MMA warp serves two CTAs, and goes on for the rest of its tile (asking it there, or the vote,
+//   took 2 % longer on 8192 x 4096 x 4096). A thread that gives up sets the flag of both CTAs first; what
+//   follows out of turn comes after that, and warp 11 looks at its flag behind each wait.
+template <bool PAIR>
+__device__ __forceinline__ bool f8_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, const F8Args& a) {
   uint64_t t0 = 0;
-  for (uint32_t n = 1; !f8_try(bar, parity); ++n) {
+  for (uint32_t n = 1; !(PAIR ? f8_try(bar, parity) : static_cast<bool>(__all_sync(0xffffffffu, f8_try(bar, parity)))); ++n) {
     if (n & 255) continue;
-    if (*abort_flag) return;
-    const uint64_t now = global_ns();
-    if (t0 == 0) t0 = now;
-    if (now - t0 > kWaitNs) {
-      *abort_flag = 1;
-      if (err) atomicOr(err, static_cast<uint32_t>(kErrMmaTimeout));
-      return;
+    bool over = *abort_flag;
+    if (!over) {
+      const uint64_t now = global_ns();
+      if (t0 == 0) t0 = now;
+      over = now - t0 > a.wait_ns;
+      if (over && a.err) atomicOr(a.err, static_cast<uint32_t>(kErrMmaTimeout));
     }
+    if (PAIR ? over : static_cast<bool>(__any_sync(0xffffffffu, over))) {
+      f8_give_up<PAIR>(abort_flag);
+      return false;
+    }
+  }
+  return true;
+}
+// What warp 11 does once a call is given up: the epilogue's barriers from the `next`-th on (four per two
+// k-blocks, in order), so that the epilogue comes to its end. A barrier is arrived at again only when the
+// epilogue has passed its last use, which `passed` counts: a second arrival before that would complete a
+// phase in place of an epilogue warp, whose bar.sync would then wait for good. (Until the call is given up
+// the two keep step by themselves: an accumulator is full again only when the epilogue has released it.)
+// The wait here comes without any copy or MMA; it is bounded by tries, not by the clock, which runs on while the GPU serves another process.
+// (A loop of its own behind the other: as part of that one the product took 5 % longer.)
+constexpr uint32_t kF8DrainTries = 1u << 24;
+template <int ACC, int COUNT>
+__device__ __forceinline__ void f8_drain(uint32_t passed, uint32_t next, uint32_t end) {
+  for (; next < end; ++next) {
+    const uint32_t ac = next % ACC, use = next / ACC;  // a fresh barrier counts as past parity 1
+    for (uint32_t n = 0; n < kF8DrainTries && !f8_try(passed + 8 * ac, (use & 1) ^ 1); ++n) {
+    }
+    __syncwarp();
+#pragma unroll
+    for (int p = 0; p < 2; ++p) asm volatile("bar.arrive %0, %1;" ::"r"(1 + ACC * p + ac), "n"(COUNT) : "memory");
   }
 }
 // One lane of a converged warp, chosen so that the compiler knows it is one: the operands of the
@@ -294,6 +338,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
   uint64_t* t_empty = t_full + kF8Acc;                    // [kF8Acc] (the leader's counts for the pair)
   uint64_t* f_full = t_empty + kF8Acc;                    // [kF8Ring]
   uint64_t* f_empty = f_full + kF8Ring;                   // [kF8Ring]
+  uint64_t* passed = f_empty + kF8Ring;                   // [kF8Acc] (this CTA's epilogue)
   unsigned char* stages = f8_smem + 1024;                 // [kF8Stages][x rows | weight block]
   float2* ring = reinterpret_cast<float2*>(stages + kF8Stages * static_cast<size_t>(kF8StageBytes));  // [kF8Ring][kF8Group][kF8Rows]
   unsigned char* out_buf = reinterpret_cast<unsigned char*>(ring + kF8Ring * kF8Group * kF8Rows);    // output rows of 8 warps
@@ -318,13 +363,15 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
     for (int i = 0; i < kF8Acc; ++i) {
       mbar_init(&t_full[i], 1);
       mbar_init(&t_empty[i], 2 * kF8EpiWarps);
+      mbar_init(&passed[i], kF8EpiWarps);
     }
     for (int i = 0; i < kF8Ring; ++i) {
       mbar_init(&f_full[i], 1);
       mbar_init(&f_empty[i], kF8EpiWarps);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    s_abort = 0;
+    s_abort = a.wait_ns == 0;
+    if (a.wait_ns == 0 && a.err) atomicOr(a.err, static_cast<uint32_t>(kErrMmaTimeout));
   }
   tc_fence_before();
   __syncthreads();
@@ -351,7 +398,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
     return t;
   };
   auto wait = [&](uint64_t* bars, int i, uint32_t parity) {  // a fresh barrier counts as past parity 1
-    f8_wait(smem_addr(bars) + 8 * i, parity, abort_flag, a.err);
+    return f8_wait<true>(smem_addr(bars) + 8 * i, parity, abort_flag, a);
   };
   auto stopped = [&]() { return __any_sync(0xffffffffu, *abort_flag); };
 
@@ -367,8 +414,8 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
         const int wrow = (2 * t.ni + static_cast<int>(rank)) * kFp8Block;
         const int xrow = t.mi * kF8PairRows + static_cast<int>(rank) * kF8Rows;
         for (int kb = 0; kb < kblocks; ++kb, (++st == kF8Stages ? (st = 0, past ^= 1) : 0)) {
-          wait(empty, st, past);
-          if (f8_elect()) {
+          const bool free = wait(empty, st, past);
+          if (f8_elect() && free) {
             unsigned char* sx = stages + static_cast<size_t>(st) * kF8StageBytes;
             const uint32_t bar = f8_of_rank(&full[st], 0);
             if (rank == 0) mbar_expect_tx(&full[st], bytes);
@@ -455,33 +502,44 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
       }
     } else {
       // ---- accumulators (and their factors) done: let the epilogue go ------------------------------
-      // It and the epilogue run through every tile even after an abort, without waiting then: a
-      // named barrier's counts have to match.
       // The factors of k-block kb + 1 are there when the epilogue passes the barrier of (kb, 1).
       int sl = 0, sph = 0, buf = 0, ph = 0;
       auto factors = [&](int kb) {
         if (kb & (kF8Group - 1)) return;
-        if (!*abort_flag) wait(f_full, sl, sph);
+        wait(f_full, sl, sph);
         if (++sl == kF8Ring) {
           sl = 0;
           sph ^= 1;
         }
       };
-      for (int tile = pair; tile < ntiles; tile += npairs) {
+      uint32_t gone = 0;  // k-blocks of the tiles before this one
+      bool given_up = a.wait_ns == 0;
+      int kb = 0, h = 0;
+      for (int tile = pair; tile < ntiles && !given_up; tile += npairs) {
         factors(0);
-        for (int kb = 0; kb < kblocks; ++kb) {
+        for (kb = 0; kb < kblocks; ++kb) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (h = 0; h < 2; ++h) {
             if (h == 1 && kb + 1 < kblocks) factors(kb + 1);
-            if (!*abort_flag) wait(t_full, 2 * buf + h, ph);
+            wait(t_full, 2 * buf + h, ph);
             __syncwarp();
+            given_up = *abort_flag;  // 0.5 % of 8192 x 4096 x 4096
+            if (given_up) break;
 #pragma unroll
             for (int p = 0; p < 2; ++p)
               asm volatile("bar.arrive %0, %1;" ::"r"(1 + kF8Acc * p + 2 * buf + h), "n"(32 * (kF8EpiWarps / 2 + 1)) : "memory");
           }
+          if (given_up) break;
           ph ^= buf;
           buf ^= 1;
         }
+        if (!given_up) gone += kblocks;
+      }
+      if (given_up) {
+        f8_give_up<true>(abort_flag);
+        const uint32_t tiles = pair < ntiles ? (ntiles - pair + npairs - 1) / npairs : 0;
+        f8_drain<kF8Acc, 32 * (kF8EpiWarps / 2 + 1)>(smem_addr(passed), a.wait_ns == 0 ? 0 : 2 * (gone + kb) + h,
+                                                     2 * tiles * kblocks);
       }
     }
   } else {
@@ -491,7 +549,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
     const int warp_row = (warp & 3) * 32, row = warp_row + lane;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp_row) << 16);
     const int col0 = part * 64, col1 = col0 + 32;
-    const uint32_t released = f8_of_rank(&t_empty[0], 0);
+    const uint32_t released = lane == 0 ? f8_of_rank(&t_empty[0], 0) : f8_of_rank(&passed[0], rank);
     unsigned char* buf_out = out_buf + warp * kF8StoreBytes;
     int buf = 0, sl = 0;
     // The two column parts go by barriers of their own: warps w and w + 4 share a scheduler, and one
@@ -503,7 +561,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
     auto release = [&](int ac) {
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) f8_arrive_remote(released + 8 * ac);
+      if (lane < 2) f8_arrive_remote(released + 8 * ac);
     };
     auto group_read = [&](int kb) {  // this warp has the factors of k-block kb: its group's last?
       if ((kb & (kF8Group - 1)) == kF8Group - 1 || kb == kblocks - 1) {

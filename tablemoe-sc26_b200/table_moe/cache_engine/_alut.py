@@ -124,6 +124,7 @@ SIGNATURES = {
     "alut_linear_fp8_workspace_size": (_SZ, [_I32, _I32, _I32]),
     "alut_linear_fp8": (ctypes.c_int, [_I32, _I32, _I32, _P, _I32, _I64, _P, _I64, _P, _P, _I32, _I64, _P, _P, _SZ,
                                        _P]),
+    "alut_set_wait_limit": (ctypes.c_int, [ctypes.c_uint64]),
     "alut_experts_fp8_workspace_size": (_SZ, [_EP, _I32, _I32]),
     "alut_experts_fp8": (ctypes.c_int, [_EP, _I32, _I32, _P, _I32, _I64, _P, _I64, _P, _I64, _I32, _P, _I32, _I64,
                                         _I64, _P, _P, _SZ, _P]),
