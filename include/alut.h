@@ -331,8 +331,9 @@ typedef enum alut_keep_mode {
   ALUT_KEEP_IMPORTANCE = 1, /* build_prefill_keep_mask (pruning.py:18-48) */
 } alut_keep_mode_t;
 
-/* Bytes of the workspace of alut_route for num_experts experts (zero-filled once; the
- * kernels leave it zeroed). 0 for invalid sizes. */
+/* Bytes of the workspace of alut_route, alut_route_experts and alut_keep_mask with
+ * ALUT_KEEP_IMPORTANCE for num_experts experts (16-byte aligned; its contents do not matter before
+ * or after a call, and calls that may run at the same time need one each). 0 for invalid sizes. */
 size_t alut_route_workspace_size(int32_t num_experts);
 
 /* Top-k softmax routing and keep mask of q tokens in one call:

@@ -609,6 +609,39 @@ static bool combine_vec(const alut_tables_t* t, const void* out, int64_t out_str
          (t->value_stride[2] * vsz) % 16 == 0 && (out_stride * osz) % 16 == 0;
 }
 
+// ---- routing ---------------------------------------------------------------------------
+
+static void place_sums(RouteArgs& a, void* workspace) {
+  a.sums = static_cast<unsigned long long*>(workspace);
+  a.counts = reinterpret_cast<int*>(static_cast<char*>(workspace) + align256(sizeof(unsigned long long) * a.e));
+}
+// The importance mode: sums cleared, the kernel that adds to them, ranking and masks, each launched as a
+// dependent of the one before.
+template <typename Args>
+static int launch_importance(void (*kern)(Args), const Args& x, const RouteArgs& a, dim3 grid, dim3 block, size_t smem,
+                             const char* what, cudaStream_t st) {
+  const size_t ks = (sizeof(long long) + sizeof(int) + 1) * static_cast<size_t>(a.e);
+  int rc = allow_smem(reinterpret_cast<const void*>(k_route_keep), ks);
+  if (rc) return rc;
+  k_route_clear<<<1, kRouteKeepThreads, 0, st>>>(a);
+  rc = check_launch("k_route_clear");
+  if (rc) return rc;
+  cudaError_t e = launch_pdl(kern, grid, block, smem, st, x);
+  if (e == cudaSuccess) e = launch_pdl(k_route_keep, dim3(1), dim3(kRouteKeepThreads), ks, st, a);
+  if (e != cudaSuccess) return fail(ALUT_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+  return ALUT_OK;
+}
+// A routing kernel of a warp per token, in either keep mode.
+template <typename Args>
+static int launch_route(void (*kern)(Args), const Args& x, const RouteArgs& a, size_t smem, const char* what, cudaStream_t st) {
+  const int rc = allow_smem(reinterpret_cast<const void*>(kern), smem);
+  if (rc) return rc;
+  const dim3 grid(ceil_div(a.q, kRouteWarps)), block(kRouteWarps * 32);
+  if (a.mode == ALUT_KEEP_IMPORTANCE) return launch_importance(kern, x, a, grid, block, smem, what, st);
+  kern<<<grid, block, smem, st>>>(x);
+  return check_launch(what);
+}
+
 }  // namespace alut
 
 using namespace alut;
@@ -789,22 +822,9 @@ int alut_route(int32_t q, int32_t num_experts, int32_t top_k, const void* logits
   a.compute = compute;
   a.reuse = reuse;
   a.out_stride = out_stride;
-  if (workspace) {
-    a.sums = static_cast<unsigned long long*>(workspace);
-    a.counts = reinterpret_cast<int*>(static_cast<char*>(workspace) + align256(sizeof(unsigned long long) * num_experts));
-  }
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const size_t sm = sizeof(float) * kRouteWarps * num_experts;
-  int rc = allow_smem(reinterpret_cast<const void*>(k_route_topk), sm);
-  if (rc) return rc;
-  k_route_topk<<<ceil_div(q, kRouteWarps), kRouteWarps * 32, sm, st>>>(a);
-  rc = check_launch("k_route_topk");
-  if (rc || keep_mode != ALUT_KEEP_IMPORTANCE) return rc;
-  const size_t ks = (sizeof(long long) + sizeof(int) + 1) * static_cast<size_t>(num_experts);
-  rc = allow_smem(reinterpret_cast<const void*>(k_route_keep), ks);
-  if (rc) return rc;
-  k_route_keep<<<1, kRouteKeepThreads, ks, st>>>(a);
-  return check_launch("k_route_keep");
+  place_sums(a, workspace);
+  return launch_route(k_route_topk, a, a, sizeof(float) * kRouteWarps * num_experts, "k_route_topk",
+                      reinterpret_cast<cudaStream_t>(stream));
 }
 
 int alut_route_experts(const alut_router_t* router, int32_t q, const void* logits, int32_t logits_dtype,
@@ -855,10 +875,7 @@ int alut_route_experts(const alut_router_t* router, int32_t q, const void* logit
   a.compute = compute;
   a.reuse = reuse;
   a.out_stride = out_stride;
-  if (workspace) {
-    a.sums = static_cast<unsigned long long*>(workspace);
-    a.counts = reinterpret_cast<int*>(static_cast<char*>(workspace) + align256(sizeof(unsigned long long) * E));
-  }
+  place_sums(a, workspace);
   x.bias = router->bias;
   x.sigmoid = router->scoring == ALUT_SCORE_SIGMOID;
   x.n_group = G;
@@ -873,17 +890,7 @@ int alut_route_experts(const alut_router_t* router, int32_t q, const void* logit
                                    : E <= 128 ? k_route_experts<4>
                                    : E <= 256 ? k_route_experts<8>
                                               : k_route_experts<0>;
-  const size_t sm = sizeof(float) * 2 * kRouteWarps * E;
-  int rc = allow_smem(reinterpret_cast<const void*>(kern), sm);
-  if (rc) return rc;
-  kern<<<ceil_div(q, kRouteWarps), kRouteWarps * 32, sm, st>>>(x);
-  rc = check_launch("k_route_experts");
-  if (rc || keep_mode != ALUT_KEEP_IMPORTANCE) return rc;
-  const size_t ks = (sizeof(long long) + sizeof(int) + 1) * static_cast<size_t>(E);
-  rc = allow_smem(reinterpret_cast<const void*>(k_route_keep), ks);
-  if (rc) return rc;
-  k_route_keep<<<1, kRouteKeepThreads, ks, st>>>(a);
-  return check_launch("k_route_keep");
+  return launch_route(kern, x, a, sizeof(float) * 2 * kRouteWarps * E, "k_route_experts", st);
 }
 
 int alut_keep_mask(int32_t q, int32_t num_experts, int32_t top_k, const int64_t* sel, const float* weights,
@@ -911,18 +918,10 @@ int alut_keep_mask(int32_t q, int32_t num_experts, int32_t top_k, const int64_t*
   a.compute = compute;
   a.reuse = reuse;
   a.out_stride = out_stride;
-  a.sums = static_cast<unsigned long long*>(workspace);
-  a.counts = reinterpret_cast<int*>(static_cast<char*>(workspace) + align256(sizeof(unsigned long long) * num_experts));
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  place_sums(a, workspace);
   const int64_t n = static_cast<int64_t>(q) * top_k;
-  k_route_scores<<<static_cast<unsigned>((n + 255) / 256), 256, 0, st>>>(a);
-  int rc = check_launch("k_route_scores");
-  if (rc) return rc;
-  const size_t ks = (sizeof(long long) + sizeof(int) + 1) * static_cast<size_t>(num_experts);
-  rc = allow_smem(reinterpret_cast<const void*>(k_route_keep), ks);
-  if (rc) return rc;
-  k_route_keep<<<1, kRouteKeepThreads, ks, st>>>(a);
-  return check_launch("k_route_keep");
+  return launch_importance(k_route_scores, a, a, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, "k_route_scores",
+                           reinterpret_cast<cudaStream_t>(stream));
 }
 
 int alut_normalize_rows(int64_t rows, int32_t l, const void* src, int64_t src_stride, void* dst, int64_t dst_stride,

@@ -24,8 +24,12 @@
 //    expert's sum as a fixed-point integer (2^-40 units, 64-bit atomics), so the sums - and
 //    with them the ranking - do not depend on the order of the additions.
 //  * k_route_keep (importance mode only, one CTA): ranks the activated experts (larger
-//    sum first, lower id on equal sums), marks the kept ones, writes the masks of every
-//    slot and clears the sums for the next call.
+//    sum first, lower id on equal sums), marks the kept ones and writes the masks of every
+//    slot.
+// A call clears its sums itself (k_route_clear), so nothing is handed from call to call and calls on
+// different streams (or in graphs) need only workspaces of their own. The three launches of the
+// importance mode overlap: each waits for the one before where it first needs its results (1 token of
+// 128 experts 9.2 us, with a memset and full launches 12.3).
 #pragma once
 
 #include "alut_common.cuh"
@@ -52,8 +56,8 @@ struct RouteArgs {
   uint8_t* compute;
   uint8_t* reuse;
   int64_t out_stride;
-  unsigned long long* sums;  // [E] fixed-point expert sums (importance mode; zero on entry)
-  int* counts;               // [E] slots routed to each expert (importance mode; zero on entry)
+  unsigned long long* sums;  // [E] fixed-point expert sums (importance mode; zero before the kernels)
+  int* counts;               // [E] slots routed to each expert (importance mode; zero before the kernels)
 };
 
 __device__ __forceinline__ float logit_at(const RouteArgs& a, int64_t t, int j) {
@@ -63,7 +67,17 @@ __device__ __forceinline__ float logit_at(const RouteArgs& a, int64_t t, int j) 
   return static_cast<const float*>(a.logits)[o];
 }
 
+// Every call of the importance mode begins with it.
+__global__ void __launch_bounds__(kRouteKeepThreads) k_route_clear(RouteArgs a) {
+  pdl_launch_dependents();
+  for (int e = threadIdx.x; e < a.e; e += kRouteKeepThreads) {
+    a.sums[e] = 0ull;
+    a.counts[e] = 0;
+  }
+}
+
 __global__ void __launch_bounds__(kRouteWarps * 32) k_route_topk(RouteArgs a) {
+  if (a.mode != ALUT_KEEP_FIXED) pdl_launch_dependents();  // (a call's last kernel lets nobody ahead)
   extern __shared__ float probs[];  // [kRouteWarps][E]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * kRouteWarps + warp;
@@ -126,6 +140,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) k_route_topk(RouteArgs a) {
     for (int s = 0; s < a.k; ++s) tot += s_w[warp][s];
     tot = fmaxf(tot, 1e-20f);  // (the sum of NaN weights too: they stay NaN)
   }
+  if (a.mode != ALUT_KEEP_FIXED) pdl_wait();  // the sums are clear
   for (int s = lane; s < a.k; s += 32) {
     float wv = s_w[warp][s];
     const int64_t e = s_i[warp][s];
@@ -148,6 +163,8 @@ __global__ void __launch_bounds__(kRouteWarps * 32) k_route_topk(RouteArgs a) {
 
 // Importance sums of given routing (alut_keep_mask): one thread per slot.
 __global__ void k_route_scores(RouteArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();  // the sums are clear
   const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (i >= static_cast<int64_t>(a.q) * a.k) return;
   const int64_t t = i / a.k;
@@ -167,6 +184,7 @@ __global__ void __launch_bounds__(kRouteKeepThreads) k_route_keep(RouteArgs a) {
   uint8_t* s_kept = reinterpret_cast<uint8_t*>(s_act + a.e);                   // [E]
   __shared__ int s_nact;
   const int tid = threadIdx.x;
+  pdl_wait();  // the sums, weights and expert ids are there
   if (tid == 0) s_nact = 0;
   __syncthreads();
   int local = 0;
@@ -175,8 +193,6 @@ __global__ void __launch_bounds__(kRouteKeepThreads) k_route_keep(RouteArgs a) {
     const int act = a.counts[e] > 0;
     s_act[e] = act;
     local += act;
-    a.sums[e] = 0ull;  // ready for the next call
-    a.counts[e] = 0;
   }
   atomicAdd(&s_nact, local);
   __syncthreads();

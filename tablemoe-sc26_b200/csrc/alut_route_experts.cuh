@@ -45,6 +45,7 @@ template <int NV>
 __global__ void __launch_bounds__(kRouteWarps * 32) k_route_experts(RouteExpertsArgs a) {
   extern __shared__ float rx_smem[];  // [kRouteWarps][scores E | ordered keys E]
   constexpr unsigned kAll = 0xffffffffu;
+  if (a.r.mode != ALUT_KEEP_FIXED) pdl_launch_dependents();  // (a call's last kernel lets nobody ahead)
   const int E = a.r.e;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * kRouteWarps + warp;
@@ -169,6 +170,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) k_route_experts(RouteExperts
     w0 /= tot;
     w1 /= tot;
   }
+  if (a.r.mode != ALUT_KEEP_FIXED) pdl_wait();  // the sums are clear
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int s = lane + 32 * h;

@@ -11,24 +11,24 @@ fallback: the logits must be CUDA tensors and the library must load.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from ..cache_engine import _alut
 
-_WORKSPACES = {}
-
-
 def _workspace(device, num_experts):
-    """Zeroed once per (device, expert count); the kernels leave it zeroed."""
-    key = (device, num_experts)
-    ws = _WORKSPACES.get(key)
-    if ws is None:
-        n = int(_alut.load().alut_route_workspace_size(num_experts))
-        if n == 0:
-            raise ValueError(f"unsupported expert count {num_experts}")
-        ws = torch.zeros(n, dtype=torch.uint8, device=device)
-        _WORKSPACES[key] = ws
-    return ws
+    """The importance mode's scratch of one call: calls on other streams, in other threads or in
+    graphs have theirs. The library clears it on the call's stream."""
+    return torch.empty_strided((_workspace_bytes(num_experts),), (1,), dtype=torch.uint8, device=device)
+
+
+@functools.cache
+def _workspace_bytes(num_experts):
+    n = int(_alut.load().alut_route_workspace_size(num_experts))
+    if n == 0:
+        raise ValueError(f"unsupported expert count {num_experts}")
+    return n
 
 
 def _check_logits(router_logits):
@@ -54,15 +54,17 @@ def route_for_lookup(router_logits, top_k, *, normalize_topk=False, keep="fixed"
     comp = torch.empty(q, top_k, dtype=torch.bool, device=dev)
     reuse = torch.empty(q, top_k, dtype=torch.bool, device=dev)
     mode = {"fixed": 0, "importance": 1}[keep]
-    attn = None
-    if mode == 1 and attn_scores is not None and attn_scores.numel() == q:
-        attn = attn_scores.reshape(-1).to(device=dev, dtype=torch.float32).contiguous()
-    ws = _workspace(dev, e)
+    attn, ws, ws_bytes = None, None, 0
+    if mode == 1:
+        if attn_scores is not None and attn_scores.numel() == q:
+            attn = attn_scores.reshape(-1).to(device=dev, dtype=torch.float32).contiguous()
+        ws = _workspace(dev, e)
+        ws_bytes = ws.numel()
     kk = -1 if keep_k is None else int(keep_k)
     rc = _alut.load().alut_route(q, e, int(top_k), x.data_ptr(), _alut.dtype_code(x.dtype), x.stride(0),
                                  int(bool(normalize_topk)), mode, max(kk, 0) if kk >= 0 else -1, float(keep_rate),
                                  _alut.ptr(attn), w.data_ptr(), sel.data_ptr(), comp.data_ptr(), reuse.data_ptr(),
-                                 top_k, ws.data_ptr(), ws.numel(), _alut.stream_ptr(dev))
+                                 top_k, _alut.ptr(ws), ws_bytes, _alut.stream_ptr(dev))
     _alut.check(rc, "alut_route")
     return w, sel, comp, reuse
 

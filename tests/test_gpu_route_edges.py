@@ -4,7 +4,8 @@ streams and in graphs: ``route_for_lookup`` / ``qwen_topk_softmax`` (softmax top
 import pytest
 import torch
 
-from table_moe.ops import qwen_topk_softmax, route_for_lookup
+from table_moe.ops import qwen_topk_softmax, route_experts, route_for_lookup
+from table_moe.skip import build_prefill_keep_mask
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda:0")
@@ -50,3 +51,68 @@ def test_softmax_router_masks_hold_on_such_rows(dtype):
         w, sel, comp, reuse = route_for_lookup(x, 6, **kw)
         assert ((sel >= 0) & (sel < 64)).all() and torch.equal(reuse, ~comp)
     assert torch.equal(route_for_lookup(x, 6, keep_k=2)[2], (torch.arange(6, device=DEV) < 2).expand(40, 6))
+
+
+def _importance(kind):
+    """A call of importance mode on logits, and the masks that it returns."""
+    if kind == "softmax":
+        return lambda x: route_for_lookup(x, 6, keep="importance", keep_rate=0.4)[2:]
+    if kind == "experts":
+        return lambda x: route_experts(x, 6, scoring="sigmoid", keep="importance", keep_rate=0.4)[2:]
+
+    def mask(x):
+        w, sel = x.topk(6, dim=-1)
+        keep = build_prefill_keep_mask(sel, w.sigmoid(), None, x.shape[1], 0.4)
+        return keep, ~keep
+    return mask
+
+
+@pytest.mark.parametrize("kind", ["softmax", "experts", "mask"])
+def test_importance_masks_of_calls_on_two_streams(kind):
+    """Each call's sums are its own: calls with other experts in favour, at the same time on other
+    streams, return what they return alone."""
+    call, e, n = _importance(kind), 96, 40
+    xs = [logits_of(3000, e, s) + torch.linspace(-2, 2, e, device=DEV).roll(31 * s) for s in (1, 2, 3)]
+    want = [call(x) for x in xs]
+    assert not torch.equal(want[0][0], want[1][0])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[] for _ in xs]
+    for _ in range(n):
+        for x, st, g in zip(xs, streams, got):
+            with torch.cuda.stream(st):
+                g.append(call(x))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, w[0]) and torch.equal(b, w[1]) for a, b in g)
+
+
+@pytest.mark.parametrize("kind,e", [("softmax", 37), ("experts", 41), ("mask", 43)])
+def test_importance_masks_whose_first_call_is_captured(kind, e):
+    """Expert counts that no other test uses: the first call is recorded, then an eager call runs before
+    the first replay, and both are right."""
+    call = _importance(kind)
+    _importance(kind)(logits_of(50, 64, 0))  # (the kernels are loaded)
+    x, y = logits_of(500, e, 1), logits_of(700, e, 2)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(x)
+    other = torch.empty(1 << 20, dtype=torch.uint8, device=DEV).fill_(255)  # memory that is not zero
+    del other
+    eager = call(y)
+    graph.replay()
+    again = call(y)
+    x0 = x.clone()
+    x.copy_(logits_of(500, e, 3))
+    graph.replay()
+    torch.cuda.synchronize()
+    second = [t.clone() for t in out]
+    x.copy_(x0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(eager, again))
+    assert all(torch.equal(a, b) for a, b in zip(out, call(x0)))
+    assert all(torch.equal(a, b) for a, b in zip(second, call(logits_of(500, e, 3))))
+    want = call(torch.cat([y]))
+    assert all(torch.equal(a, b) for a, b in zip(eager, want))
