@@ -38,6 +38,7 @@ namespace alut {
 
 constexpr int kRouteWarps = 4;                 // tokens per CTA of k_route_topk
 constexpr int kRouteKeepThreads = 1024;
+constexpr float kRouteNan = -0.5f;             // ranks a NaN among the probabilities of a token
 constexpr int kRouteMaxExperts = kMaxTables;   // probabilities of a token in shared memory
 constexpr double kRouteFixedScale = 1099511627776.0;  // 2^40
 
@@ -100,10 +101,13 @@ __global__ void __launch_bounds__(kRouteWarps * 32) k_route_topk(RouteArgs a) {
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  for (int j = lane; j < a.e; j += 32) p[j] = sum == 0.f ? 0.f : p[j] / sum;
+  for (int j = lane; j < a.e; j += 32) {
+    const float v = sum == 0.f ? 0.f : p[j] / sum;
+    p[j] = isnan(v) ? kRouteNan : v;
+  }
   __syncwarp();
   // top_k <= E rounds of arg-max; the chosen entry is retired with -1. Probabilities are >= 0 and
-  // a NaN counts as -0.5, so every round finds an entry that is not retired: bi is an expert's.
+  // kRouteNan is above -1, so every round finds an entry that is not retired: bi is an expert's.
   __shared__ float s_w[kRouteWarps][kMaxSlots];
   __shared__ int s_i[kRouteWarps][kMaxSlots];
   for (int s = 0; s < a.k; ++s) {
@@ -111,9 +115,8 @@ __global__ void __launch_bounds__(kRouteWarps * 32) k_route_topk(RouteArgs a) {
     int bi = 0x7fffffff;
     for (int j = lane; j < a.e; j += 32) {
       const float v = p[j];
-      const float key = isnan(v) ? -0.5f : v;
-      if (key > bv) {  // ascending j per lane: the lane's first maximum is kept
-        bv = key;
+      if (v > bv) {  // ascending j per lane: the lane's first maximum is kept
+        bv = v;
         bi = j;
       }
     }
@@ -127,9 +130,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32) k_route_topk(RouteArgs a) {
       }
     }
     if (lane == 0) {
-      s_w[warp][s] = p[bi];
-      s_i[warp][s] = bi;
       p[bi] = -1.f;
+      s_w[warp][s] = bv == kRouteNan ? NAN : bv;
+      s_i[warp][s] = bi;
     }
     __syncwarp();
   }
