@@ -347,7 +347,8 @@ size_t alut_route_workspace_size(int32_t num_experts);
  *     ALUT_KEEP_IMPORTANCE: expert sel[t, s] is among the first max(1, int(n_active *
  *       keep_rate)) activated experts ranked by the sum over their slots of
  *       attn[t] * weights[t, s] (attn != NULL) or weights[t, s] / q (larger sum first, lower
- *       id on equal sums; sums are accumulated exactly in 2^-40 fixed point, |sum| < 2^23).
+ *       id on equal sums; sums are accumulated exactly in 2^-40 fixed point, |sum| < 2^23, and a
+ *       NaN adds 0 to them).
  * Outputs are [q, top_k] with row stride out_stride (elements). top_k <= 64 and
  * top_k <= num_experts <= 4096. Replaces qwen_topk_softmax followed by _build_compute_mask
  * (qwen3_vl_moe/cached_layers.py:69-84, :282-286, :336). */

@@ -68,6 +68,14 @@ __device__ __forceinline__ float logit_at(const RouteArgs& a, int64_t t, int j) 
   return static_cast<const float*>(a.logits)[o];
 }
 
+// A slot's score, added to its expert's sum. A NaN counts as 0: as a fixed-point number it would be the
+// lowest there is, and its expert would come last for the whole batch.
+__device__ __forceinline__ void add_score(const RouteArgs& a, int64_t e, float score) {
+  if (!isnan(score))
+    atomicAdd(&a.sums[e], static_cast<unsigned long long>(__double2ll_rn(static_cast<double>(score) * kRouteFixedScale)));
+  atomicAdd(&a.counts[e], 1);
+}
+
 // Every call of the importance mode begins with it.
 __global__ void __launch_bounds__(kRouteKeepThreads) k_route_clear(RouteArgs a) {
   pdl_launch_dependents();
@@ -156,10 +164,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) k_route_topk(RouteArgs a) {
       a.reuse[t * a.out_stride + s] = comp ? 0 : 1;
     } else {
       // pruning.py:29-35: attn_scores[t] * w, else w / max(Q, 1) (fp32), summed per expert.
-      const float score = a.attn ? a.attn[t] * wv : wv / static_cast<float>(max(a.q, 1));
-      const long long fx = __double2ll_rn(static_cast<double>(score) * kRouteFixedScale);
-      atomicAdd(&a.sums[e], static_cast<unsigned long long>(fx));
-      atomicAdd(&a.counts[e], 1);
+      add_score(a, e, a.attn ? a.attn[t] * wv : wv / static_cast<float>(max(a.q, 1)));
     }
   }
 }
@@ -175,9 +180,7 @@ __global__ void k_route_scores(RouteArgs a) {
   const int64_t e = a.sel[t * a.out_stride + s];
   if (e < 0 || e >= a.e) return;  // rejected by the keep kernel's range check below
   const float wv = a.w[t * a.out_stride + s];
-  const float score = a.attn ? a.attn[t] * wv : wv / static_cast<float>(max(a.q, 1));
-  atomicAdd(&a.sums[e], static_cast<unsigned long long>(__double2ll_rn(static_cast<double>(score) * kRouteFixedScale)));
-  atomicAdd(&a.counts[e], 1);
+  add_score(a, e, a.attn ? a.attn[t] * wv : wv / static_cast<float>(max(a.q, 1)));
 }
 
 __global__ void __launch_bounds__(kRouteKeepThreads) k_route_keep(RouteArgs a) {

@@ -185,9 +185,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) k_route_experts(RouteExperts
       a.r.compute[o] = comp ? 1 : 0;
       a.r.reuse[o] = comp ? 0 : 1;
     } else {  // the importance sums of alut_route
-      const float score = a.r.attn ? a.r.attn[t] * wv : wv / static_cast<float>(max(a.r.q, 1));
-      atomicAdd(&a.r.sums[e], static_cast<unsigned long long>(__double2ll_rn(static_cast<double>(score) * kRouteFixedScale)));
-      atomicAdd(&a.r.counts[e], 1);
+      add_score(a.r, e, a.r.attn ? a.r.attn[t] * wv : wv / static_cast<float>(max(a.r.q, 1)));
     }
   }
 }

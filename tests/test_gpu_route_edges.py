@@ -1,5 +1,4 @@
-"""The routers on rows that are not ordinary numbers, on inputs of unusual strides, and on several
-streams and in graphs: ``route_for_lookup`` / ``qwen_topk_softmax`` (softmax top-k) and
+"""The routers on rows that are not ordinary numbers, and on several streams and in graphs: ``route_for_lookup`` / ``qwen_topk_softmax`` (softmax top-k) and
 ``route_experts``."""
 import pytest
 import torch
@@ -116,3 +115,20 @@ def test_importance_masks_whose_first_call_is_captured(kind, e):
     assert all(torch.equal(a, b) for a, b in zip(second, call(logits_of(500, e, 3))))
     want = call(torch.cat([y]))
     assert all(torch.equal(a, b) for a, b in zip(eager, want))
+
+
+@pytest.mark.parametrize("bad", [1, 2, 5])
+def test_a_nan_token_does_not_decide_the_others_masks(bad):
+    """Its score adds nothing to its experts' sums: the mask is the one of weights with 0 in its place."""
+    e, k = 48, 4
+    x = logits_of(200, e, bad)
+    x[:, :k] += 3.0  # the experts that a NaN row names are the batch's most important
+    rows = torch.arange(bad, device=DEV) * 7
+    x[rows] = NAN
+    for route in (lambda **kw: route_for_lookup(x, k, **kw), lambda **kw: route_experts(x, k, scoring="softmax", **kw)):
+        for attn in (None, torch.rand(200, generator=torch.Generator().manual_seed(1)).to(DEV)):
+            w, sel, comp, _ = route(keep="importance", keep_rate=0.2, attn_scores=attn)
+            assert w[rows].isnan().all()
+            want = build_prefill_keep_mask(sel, w.nan_to_num(0.0), attn, e, 0.2)
+            assert torch.equal(comp, want) and comp[rows].all()
+            assert torch.equal(build_prefill_keep_mask(sel, w, attn, e, 0.2), want)
