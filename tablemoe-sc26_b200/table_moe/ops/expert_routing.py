@@ -38,7 +38,7 @@ def route_experts(router_logits, top_k, *, scoring="softmax", bias=None, n_group
     come last. ``normalize_topk`` divides the weights by their sum (clamped at 1e-20), then
     ``scale`` multiplies them. ``keep``, ``keep_k``, ``keep_rate``, ``attn_scores``: the keep
     mask, as in ``route_for_lookup``."""
-    x = _check_logits(router_logits)
+    x, stride = _check_logits(router_logits)
     q, e = x.shape
     dev = x.device
     top_k, n_group = int(top_k), int(n_group)
@@ -62,7 +62,7 @@ def route_experts(router_logits, top_k, *, scoring="softmax", bias=None, n_group
             attn = attn_scores.reshape(-1).to(device=dev, dtype=torch.float32).contiguous()
         ws = _workspace(dev, e)
         ws_bytes = ws.numel()
-    rc = _alut.load().alut_route_experts(r, q, x.data_ptr(), _alut.dtype_code(x.dtype), x.stride(0), mode,
+    rc = _alut.load().alut_route_experts(r, q, x.data_ptr(), _alut.dtype_code(x.dtype), stride, mode,
                                          -1 if keep_k is None else max(int(keep_k), 0), keep_rate, _alut.ptr(attn),
                                          w.data_ptr(), sel.data_ptr(), comp.data_ptr(), reuse.data_ptr(), top_k,
                                          _alut.ptr(ws), ws_bytes, _alut.stream_ptr(dev))

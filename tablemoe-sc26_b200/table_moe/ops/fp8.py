@@ -130,7 +130,7 @@ class Fp8Linear(_Fp8Module):
                 y = y.view(*x.shape[:-1], n)
             stride = n
         else:
-            if out.shape != (m, n) or out.device != x.device or out.stride(-1) != 1:
+            if out.shape != (m, n) or out.device != x.device or (n > 1 and out.stride(-1) != 1):
                 raise ValueError(f"out must be a [{m}, {n}] tensor on {x.device} with unit innermost stride")
             if out_dtype is not None and out_dtype != out.dtype:
                 raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
@@ -204,9 +204,13 @@ class Fp8Experts(_Fp8Module):
         out = collected
         if out is None:
             out = torch.empty_strided((q, s, h), (s * h, h, 1), dtype=x.dtype, device=dev)
-        elif out.shape != (q, s, h) or out.device != dev or out.stride(-1) != 1:
+        elif out.shape != (q, s, h) or out.device != dev or (h > 1 and out.stride(-1) != 1):
             raise ValueError(f"collected must be [{q}, {s}, {h}] on {dev} with unit innermost stride")
         out_t, out_s, _ = out.stride()
+        if q == 1:  # (the stride of one token, or slot, means nothing)
+            out_t = max(out_t, h)
+        if s == 1:
+            out_s = max(out_s, h)
         lib = self._lib
         nbytes = lib.alut_experts_fp8_workspace_size(self._weights, q, s)
         ws = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=dev)

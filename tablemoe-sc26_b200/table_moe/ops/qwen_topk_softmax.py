@@ -32,12 +32,16 @@ def _workspace_bytes(num_experts):
 
 
 def _check_logits(router_logits):
+    """The logits with unit innermost stride, and their row stride."""
     if router_logits.dim() != 2:
         raise ValueError(f"qwen_topk_softmax expects 2D logits, got {tuple(router_logits.shape)}")
     if router_logits.device.type != "cuda":
         raise ValueError("router logits must be a CUDA tensor (the ALUT router has no CPU path)")
-    x = router_logits if router_logits.stride(-1) == 1 else router_logits.contiguous()
-    return x
+    e = router_logits.shape[1]
+    stride, inner = router_logits.stride()
+    if inner != 1 or stride < e:  # also a broadcast row, or one row (whose stride means nothing)
+        return router_logits.contiguous(), e
+    return router_logits, stride
 
 
 def route_for_lookup(router_logits, top_k, *, normalize_topk=False, keep="fixed", keep_k=None, keep_rate=0.6,
@@ -46,7 +50,7 @@ def route_for_lookup(router_logits, top_k, *, normalize_topk=False, keep="fixed"
     reuse_mask [Q,k] bool). ``keep``: "fixed" (the first ``keep_k`` slots computed,
     build_fixed_keep_mask / build_decode_keep_mask; None keeps all) or "importance"
     (build_prefill_keep_mask with ``keep_rate`` and optional per-token ``attn_scores``)."""
-    x = _check_logits(router_logits)
+    x, stride = _check_logits(router_logits)
     q, e = x.shape
     dev = x.device
     w = torch.empty(q, top_k, dtype=torch.float32, device=dev)
@@ -61,7 +65,7 @@ def route_for_lookup(router_logits, top_k, *, normalize_topk=False, keep="fixed"
         ws = _workspace(dev, e)
         ws_bytes = ws.numel()
     kk = -1 if keep_k is None else int(keep_k)
-    rc = _alut.load().alut_route(q, e, int(top_k), x.data_ptr(), _alut.dtype_code(x.dtype), x.stride(0),
+    rc = _alut.load().alut_route(q, e, int(top_k), x.data_ptr(), _alut.dtype_code(x.dtype), stride,
                                  int(bool(normalize_topk)), mode, max(kk, 0) if kk >= 0 else -1, float(keep_rate),
                                  _alut.ptr(attn), w.data_ptr(), sel.data_ptr(), comp.data_ptr(), reuse.data_ptr(),
                                  top_k, _alut.ptr(ws), ws_bytes, _alut.stream_ptr(dev))
