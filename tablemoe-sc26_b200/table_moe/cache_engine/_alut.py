@@ -10,6 +10,7 @@ mirroring the prebuilt-extension lookup of the reference
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from pathlib import Path
 
@@ -209,6 +210,39 @@ def stream_ptr(device) -> int:
     if _raw_stream is not None and device.index is not None:
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+# ---- the GPU of a call ------------------------------------------------------------------
+# The library launches on the current GPU. A call on tensors of another one (layers placed over
+# several GPUs by one process) runs with that one current.
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def elsewhere(device) -> bool:
+    """Whether `device` is a GPU other than the current one."""
+    return device.index is not None and device.index != _current_device()
+
+
+def on_own_device(method):
+    """For methods of objects whose tensors are on ``self.device``."""
+    @functools.wraps(method)
+    def call(self, *args, **kwargs):
+        if elsewhere(self.device):
+            with torch.cuda.device(self.device):
+                return method(self, *args, **kwargs)
+        return method(self, *args, **kwargs)
+    return call
+
+
+def on_device_of_first(fn):
+    """For functions of a tensor: on its GPU."""
+    @functools.wraps(fn)
+    def call(x, *args, **kwargs):
+        if elsewhere(x.device):
+            with torch.cuda.device(x.device):
+                return fn(x, *args, **kwargs)
+        return fn(x, *args, **kwargs)
+    return call
 
 
 def _inner_contig(t: torch.Tensor, name: str) -> None:

@@ -32,6 +32,7 @@ def _resolve_cache_dtype():
     raise ValueError(f"Unsupported cache dtype: {dtype!r}")
 
 
+@_alut.on_device_of_first
 def normalize_rows(x: torch.Tensor, eps: float) -> torch.Tensor:
     """L2-normalise the last dim in fp32 with zero rows kept at zero, then cast back
     (load-time key normalisation, manager.py:24-31). CUDA tensors go through the
@@ -119,6 +120,7 @@ class HybridStorageManager:
             self.online_expert_ids = None
 
     # ---- C-ABI table descriptor ---------------------------------------------------------
+    @_alut.on_own_device
     def alut_tables(self):
         """The ``alut_tables_t`` of this layer (rebuilt when a buffer is replaced)."""
         pv, pt = self.pca["vision"], self.pca["text"]
@@ -136,6 +138,7 @@ class HybridStorageManager:
             self._tables = (key, t)
         return self._tables[1]
 
+    @_alut.on_own_device
     def prepare_tensor_core(self, keyset):
         """The tensor-core form of one key set (``_alut.KEYS_RAW`` or ``KEYS_NORMALISED``):
         made once, on the first batch large enough to use it (it takes as much memory as
@@ -262,6 +265,7 @@ class HybridStorageManager:
         return t.contiguous()
 
     @torch.no_grad()
+    @_alut.on_own_device
     def gather_values(self, expert_ids, modality_ids, cluster_ids):
         """values[e, m, c] rows for each i, a bit-exact device copy -> [n, H]."""
         e, m, c = self._ids(expert_ids), self._ids(modality_ids), self._ids(cluster_ids)
@@ -276,6 +280,7 @@ class HybridStorageManager:
         return out
 
     @torch.no_grad()
+    @_alut.on_own_device
     def gather_values_decode_bs1(self, expert_ids, modality_id, cluster_ids, slot_ids, out_buffer):
         """out_buffer[slot_ids[i]] = values[expert_ids[i], modality_id, cluster_ids[i]]."""
         e = self._ids(expert_ids).reshape(-1)

@@ -100,6 +100,7 @@ class VectorSearchEngine:
             self._alut_ws_shape = (cq, cs)
         return self._alut_ws
 
+    @_alut.on_own_device
     def device_errors(self, clear=True):
         """Device error bits (ALUT_ERR_*) accumulated in this engine's workspace since the last
         clear; synchronises the current stream."""
@@ -126,6 +127,7 @@ class VectorSearchEngine:
             }
             self.workspace_capacity = cap
 
+    @_alut.on_own_device
     def _search_into(self, hidden_states, selected_experts, is_vision_mask, reuse_mask, out_hit,
                      out_idx, *, keyset, normalize, cmp_ge, thr_vision, thr_text):
         """One alut_search call writing every (token, slot) of out_hit / out_idx."""
@@ -195,6 +197,7 @@ class VectorSearchEngine:
             return 0
         return m.online_size if m.online_full else m.online_ptr
 
+    @_alut.on_own_device
     def _search_online_into(self, hidden_states, target_eids, out_on_hit, out_on_idx, out_on_slot):
         """Online window lookup (search.py:778-806) in one kernel (``alut_online_search``):
         best of the recent tokens by dot product in the window dtype, valid iff > 0, then
@@ -292,6 +295,7 @@ class VectorSearchEngine:
                           cmp_ge=True, thr_vision=0.0, thr_text=0.0)
 
     # ---- fused lookup (search + gather + weighted accumulate) --------------------------
+    @_alut.on_own_device
     def lookup_combine(self, hidden_states, selected_experts, is_vision_mask, reuse_mask, routing_weights,
                        *, compute_mask=None, out=None, variant="prefill_dot", renorm="to_one",
                        return_hits=False, hit_out=None, idx_out=None, computed=None):

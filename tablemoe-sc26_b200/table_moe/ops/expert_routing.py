@@ -25,6 +25,7 @@ def _choice(table, value, name):
         raise ValueError(f"{name} must be one of {sorted(table)}, got {value!r}") from None
 
 
+@_alut.on_device_of_first
 def route_experts(router_logits, top_k, *, scoring="softmax", bias=None, n_group=1, topk_group=None, group_rule="max",
                   normalize_topk=False, scale=1.0, keep="fixed", keep_k=None, keep_rate=0.6, attn_scores=None):
     """(weights [Q,k] f32, selected_experts [Q,k] int64, compute_mask [Q,k] bool, reuse_mask

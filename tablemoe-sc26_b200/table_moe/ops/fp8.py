@@ -23,6 +23,7 @@ def _blocks(n):
     return -(-n // BLOCK)
 
 
+@_alut.on_device_of_first
 def quantize_fp8(x, block_rows=1):
     """(e4m3 [..., rows, cols], fp32 scales [..., ceil(rows / block_rows), ceil(cols / 128)]) of x
     (f32, bf16 or f16; at least 2D): block_rows 1 for activations, 128 for weights."""
@@ -118,6 +119,7 @@ class Fp8Linear(_Fp8Module):
         """From a weight [N, K] in f32, bf16 or f16."""
         return cls(*quantize_fp8(weight, BLOCK))
 
+    @_alut.on_own_device
     def __call__(self, x, out=None, *, out_dtype=None):
         """x [..., K] (f32, bf16 or f16) -> [..., N] in ``out_dtype`` (default x's), or into ``out``
         (a 2D tensor [rows, N] with unit innermost stride)."""
@@ -179,6 +181,7 @@ class Fp8Experts(_Fp8Module):
         """From weights [E, 2, I, H] and [E, H, I] in f32, bf16 or f16."""
         return cls(*quantize_fp8(gate_up, BLOCK), *quantize_fp8(down, BLOCK))
 
+    @_alut.on_own_device
     def __call__(self, x, selected_experts, compute_mask=None, collected=None):
         """Outputs [Q, S, H] of the experts ``selected_experts`` [Q, S] on the tokens x [Q, H], for
         the slots of ``compute_mask`` [Q, S] (None: all). Without ``collected`` a new tensor of x's

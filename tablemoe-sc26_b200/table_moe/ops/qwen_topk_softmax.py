@@ -44,6 +44,7 @@ def _check_logits(router_logits):
     return router_logits, stride
 
 
+@_alut.on_device_of_first
 def route_for_lookup(router_logits, top_k, *, normalize_topk=False, keep="fixed", keep_k=None, keep_rate=0.6,
                      attn_scores=None):
     """(weights [Q,k] f32, selected_experts [Q,k] int64, compute_mask [Q,k] bool,

@@ -28,6 +28,7 @@ def build_decode_keep_mask(selected_experts: torch.Tensor, keep_k: int | None) -
     return build_fixed_keep_mask(selected_experts, keep_k)
 
 
+@_alut.on_device_of_first
 def build_prefill_keep_mask(selected_experts, routing_weights, attn_scores, num_experts, keep_rate):
     if selected_experts.numel() == 0:
         return torch.zeros_like(selected_experts, dtype=torch.bool)
