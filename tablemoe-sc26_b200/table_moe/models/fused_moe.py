@@ -23,6 +23,7 @@ import torch
 from ..cache_engine import VectorSearchEngine
 from ..ops.expert_routing import route_experts
 from ..ops.qwen_topk_softmax import route_for_lookup
+from .fp8_moe import Fp8SharedExpert
 
 
 class ALUTCachedMoE:
@@ -37,7 +38,8 @@ class ALUTCachedMoE:
     ``router``: keyword arguments of ``table_moe.ops.route_experts`` (scoring, bias, n_group,
     topk_group, group_rule, scale) for layers that do not route by a plain softmax.
     ``shared``: a callable x -> [Q, H] whose result is added (shared experts, e.g.
-    ``Fp8SharedExpert``); called with ``out_dtype`` set to the value dtype.
+    ``Fp8SharedExpert``); called with ``out_dtype`` set to the value dtype. What it returns is not
+    changed (a ``Fp8SharedExpert``'s is the layer's own, and its output).
 
     Defaults follow the Qwen3-VL wrapper: prefill keeps experts by importance
     (``KEEP_RATE``), decode keeps the first ``decode_keep_k`` slots; prefill searches with the
@@ -76,7 +78,11 @@ class ALUTCachedMoE:
         values = self.manager.values_buffer
         collected = torch.empty((x.shape[0], self.top_k, values.shape[-1]), dtype=values.dtype, device=x.device)
         run_experts(x, sel, comp, collected)
-        base = None if self.shared is None else self.shared(x, out_dtype=values.dtype)  # the lookups add to it
+        base = None
+        if self.shared is not None:
+            base = self.shared(x, out_dtype=values.dtype)
+            if type(self.shared) is not Fp8SharedExpert:  # the lookups add to it: into a tensor of the call's
+                base = torch.empty((x.shape[0], values.shape[-1]), dtype=values.dtype, device=x.device).copy_(base)
         out = self.engine.lookup_combine(x, sel, is_vision.reshape(-1), reuse, w, compute_mask=comp,
                                          variant=self.prefill_variant if is_prefill else self.decode_variant,
                                          renorm=self.renorm, computed=collected, return_hits=return_routing, out=base)
