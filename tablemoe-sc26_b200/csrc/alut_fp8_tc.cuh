@@ -522,8 +522,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) __cluster_dims__(2, 1, 1)
           for (h = 0; h < 2; ++h) {
             if (h == 1 && kb + 1 < kblocks) factors(kb + 1);
             wait(t_full, 2 * buf + h, ph);
-            __syncwarp();
-            given_up = *abort_flag;  // 0.5 % of 8192 x 4096 x 4096
+            given_up = stopped();
             if (given_up) break;
 #pragma unroll
             for (int p = 0; p < 2; ++p)
