@@ -230,7 +230,8 @@ constexpr int kFp8MaxExperts = 2048;  // two per thread of the plan
 // through shared memory in warp order: ks = 8 where few CTAs have to hide the latency of one token,
 // less where there are enough (fewer barriers per byte).
 // The weights come by 16-byte asynchronous copies into a ring in shared memory, kStreamDepth steps
-// ahead: 64 KB in flight per CTA, two CTAs per SM (registers held a quarter of that). Every lane
+// ahead: 64 KB in flight per CTA (registers held a quarter of that), two CTAs per SM up to K = 3840
+// and one above, where x's words, 1 KB for 128 columns, take the rest. Every lane
 // copies the 16 bytes that it reads itself (4 lanes a row, both 64-byte halves of a block), so the
 // ring needs no barrier; and since a dot product may be taken in any order of k, those words are used
 // as they lie, x's in the same order. x is quantised once per CTA, by the warp that needs the block:
@@ -238,7 +239,8 @@ constexpr int kFp8MaxExperts = 2048;  // two per thread of the plan
 // shared memory. Up to 8 routed slots need no plan: an expert's first slot leads.
 // Measured, weights from HBM, one row: 2048 x 2048 5.6 us, 4096 x 4096 10.2, 150000 x 2048 58 (5.3
 // TB/s); 8 slots of 8 experts of 2048 x 768 (38 MB, two launches) 24.6. The small ones are bound by
-// latency: launch, x's form, the first weights, the reduction over warps.
+// latency: launch, x's form, the first weights, the reduction over warps. With one CTA per SM 4096 x
+// 8192 takes 18 us.
 
 constexpr int kStreamRows = 8;        // rows of x per CTA
 constexpr int kStreamWRows = 16;      // weight rows per tile, two tiles per step

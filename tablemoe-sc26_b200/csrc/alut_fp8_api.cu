@@ -36,7 +36,8 @@ static int launch_stream(StreamArgs a, int x_dtype, unsigned groups, bool pdl, c
   auto slices = [&](int ks, int steps) {
     return static_cast<int64_t>(ceil_div(a.n, static_cast<int64_t>(steps) * (kStreamWarps / ks) * rows));
   };
-  // Few CTAs: every warp a share of K, the shortest way through. Enough for two per SM: at least 3
+  // Few CTAs: every warp a share of K, the shortest way through. Two for each SM (whether or not two
+  // fit, above K = 3840 one does): at least 3
   // k-blocks a warp and up to kStreamMaxSteps steps per CTA, over which the search for the group and
   // x's form are paid once. Measured, 8 rows: 32000 x 2048 19.2 us with this and 25.3 with all warps
   // across K, 150000 x 2048 59 and 96 (71 with one step per CTA); up to 12288 x 2048 there is no difference.
@@ -160,7 +161,8 @@ static int launch_rows(const F8PrepArgs& a, int x_dtype, cudaStream_t st) {
 // 64; 12288 x 2048 12.2 / 13.9 for 8, 16.4 / 14.0 for 24; 150000 x 2048 61 / 83 for 8, 88 / 80 for 16: what is
 // read in all decides, and one pass is always streamed. Where that is little, the passes over x's form
 // do: 1024 x 1024 7.4 / 10.7 for 128, 10.4 / 10.7 for 192, 13.1 / 10.6 for 256; 2048 x 768 9.4 / 9.7 for 128,
-// 11.0 / 9.8 for 192.
+// 11.0 / 9.8 for 192. Past kStreamMaxBlocks x's words do not fit beside the ring, and few rows are left with
+// one group's ceil(n / 256) CTAs: 4096 x 8192 18.1 us for 1 row, x 8320 29.1, x 12288 40.4.
 static bool linear_streams(int m, int n, int k) {
   const int64_t passes = ceil_div(m, kStreamRows);
   return (passes == 1 || (passes <= 16 && passes * n * k <= (40ll << 20))) && fp8_blocks(k) <= kStreamMaxBlocks;
