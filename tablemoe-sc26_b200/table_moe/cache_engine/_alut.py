@@ -235,13 +235,16 @@ def on_own_device(method):
 
 
 def on_device_of_first(fn):
-    """For functions of a tensor: on its GPU."""
+    """For functions whose first argument is a tensor: on its GPU."""
+    first = fn.__code__.co_varnames[0]
+
     @functools.wraps(fn)
-    def call(x, *args, **kwargs):
-        if elsewhere(x.device):
+    def call(*args, **kwargs):
+        x = args[0] if args else kwargs.get(first)
+        if isinstance(x, torch.Tensor) and elsewhere(x.device):
             with torch.cuda.device(x.device):
-                return fn(x, *args, **kwargs)
-        return fn(x, *args, **kwargs)
+                return fn(*args, **kwargs)
+        return fn(*args, **kwargs)
     return call
 
 
